@@ -262,7 +262,7 @@ def prepare(case, seed):
         s.slots = torch.randperm(S + 2, generator=g, device=GPU)[:S].int()
     if own:
         from runtime.kernels import cache4
-        s.plan = cache4.plan(counts, cached, heads, kv, dim, window=s.window, device=GPU,
+        s.plan = cache4.plan(counts, cached, heads, kv, dim, window=s.window, device=GPU, dtype=dtype,
                              state_slots=s.slots.tolist() if s.sums is not None else None)
     return s
 
