@@ -1,0 +1,361 @@
+"""The cache that holds keys and values in 4 bits, and that may keep a bounded number of keys: its kernels' checked entry points,
+the rules that pick their forms, and the step metadata they want.
+
+A block of 32 coordinates of one token's key (value) is held as a power of two and 32 codes of 4 bits (0, 0.5, 1, 1.5, 2, 3, 4, 6 and
+their negatives times the power; csrc/cache4.h has the layout): 4.25 bits a coordinate, a quarter of the bfloat16 cache, and every
+held number is a bfloat16 as it is.  Heads of any even size up to 256, pages of a power of two from 8 tokens on, activations in bfloat16
+or float32.
+
+  rope_write    turns queries and keys, writes keys and values into the pages
+  attention     softmax attention of a step's rows over the pages (prompt portions and single tokens)
+  add_weights   adds every key's attention weight, summed over the rows and heads that see it, to what it had
+  evict         keeps of each head's keys the last ones and those with the largest sums
+  read          what the pages hold, as bfloat16
+
+`attend` is what a mixer calls.  Launches go to the current stream of the tensors' device.  A Plan's workspace belongs to one launch at a
+time: two streams need two plans.
+The reference has nothing of this kind (its cache is float32 and keeps every key, runtime/cache.py:9-118).
+"""
+import contextlib
+import ctypes as C
+import operator
+from dataclasses import dataclass, field
+from typing import Optional
+
+import numpy as np
+import torch
+
+from . import library, ops
+from .attention import fill_tasks
+from .ops import BF16, F32, KernelError
+
+UNIT = library.CACHE4
+MAX_HEAD = 256
+_DT = {torch.bfloat16: BF16, torch.float32: F32}
+_entries = {}
+
+
+def padded(dim):
+    """A head's coordinates with the zeros that fill its last block."""
+    return -(-dim // 32) * 32
+
+
+def record_bytes(dim, page_size):
+    """Bytes of one head's page, keys and values."""
+    return page_size * (padded(dim) + padded(dim) // 16)
+
+
+def supported(dim, page_size):
+    return 0 < dim <= MAX_HEAD and dim % 2 == 0 and page_size >= 8 and page_size & (page_size - 1) == 0
+
+
+def _entry(name):
+    fn = _entries.get(name)
+    if fn is None:
+        p, i, f, ll = C.c_void_p, C.c_int, C.c_float, C.c_longlong
+        kind = name.split("_d")[0]
+        fn = getattr(library.load(UNIT), name)
+        fn.argtypes = {
+            "cisr_write4": [p, p, p, p, p, p, p, i, i, i, i, i, i, i, i, i, i, p],
+            "cisr_read4": [p, p, p, p, i, i, i, i, i, i, p],
+            "cisr_evict4": [p, p, p, p, p, p, p, p, i, i, i, i, i, i, i, i, i, i, i, i, p],
+            "cisr_merge4": [p, p, p, p, i, i, i, i, p],
+            "cisr_attn4": [p, p, p, p, p, p, p, p, ll, i, i, i, i, i, i, i, i, f, i, i, i, p],
+            "cisr_weights4": [p, p, p, p, p, p, ll, i, i, i, i, i, i, i, i, i, i, f, i, i, p],
+        }[kind]
+        fn.restype = C.c_int
+        _entries[name] = fn
+    return fn
+
+
+def _t(t, name, dtype, shape, device=None, align=1):
+    """The address of a contiguous GPU tensor of that type and shape (on `device`, on so many bytes)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise KernelError(f"{name}: expected a GPU tensor")
+    if t.dtype != dtype:
+        raise KernelError(f"{name}: dtype {t.dtype}, expected {dtype}")
+    if t.shape != shape:
+        raise KernelError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if not t.is_contiguous():
+        raise KernelError(f"{name}: tensor must be contiguous")
+    if device is not None and t.device != device:
+        raise KernelError(f"{name}: on {t.device}, the others on {device}")
+    at = t.data_ptr()
+    if at % align:
+        raise KernelError(f"{name}: must lie on {align} bytes")
+    return at
+
+
+def _geometry(heads, kv_heads, dim, page_size):
+    if not supported(dim, page_size):
+        raise KernelError(f"cache4: heads of {dim} in pages of {page_size}: an even size up to {MAX_HEAD}, a power of two from 8 on")
+    if kv_heads <= 0 or heads <= 0 or heads % kv_heads:
+        raise KernelError(f"cache4: {heads} query heads are not a multiple of {kv_heads} key/value heads")
+
+
+def _pages(pages, kv_heads, dim, page_size, name="pages"):
+    """(address, pages) of one site's pages [n, kv_heads, bytes]."""
+    if not isinstance(pages, torch.Tensor) or pages.dim() != 3 or not 0 < pages.shape[0] < 1 << 31:
+        raise KernelError(f"{name}: expected pages of one site, [n, kv_heads, bytes]")
+    return _t(pages, name, torch.uint8, (pages.shape[0], kv_heads, record_bytes(dim, page_size)), None, 16), pages.shape[0]
+
+
+def _on(device):
+    """The tensors' device as the current one, for the launch (their stream is that device's current one)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _launch(name, device, *args):
+    with _on(device):
+        code = _entry(name)(*args, ops._stream())
+    if code:
+        raise KernelError(f"{name}: HIP error {code}")
+
+
+def _scale(scale):
+    scale = float(scale)
+    if not 0.0 < scale < float("inf"):
+        raise KernelError(f"cache4: the score scale must be positive, not {scale}")
+    return scale
+
+
+def _window(window):
+    window = operator.index(window or 0)
+    if not 0 <= window < 1 << 31:
+        raise KernelError(f"cache4: a window of {window} keys")
+    return window
+
+
+# -- writing and reading ------------------------------------------------------------------------------------------
+
+def rope_write(qkv, positions, slots, cos, sin, pages, q, heads, kv_heads, dim, page_size, interleaved=False):
+    """Turns queries and keys of the fused projection rows qkv [T, (heads + 2 kv_heads) dim] by the angles of `positions` int32 [T]
+    (cos, sin float [max_pos, rot / 2]; pair i of a head is coordinates (i, i + rot / 2), or with `interleaved` (2 i, 2 i + 1)), puts
+    the queries into q [T, heads dim] and holds keys and values in the token slots `slots` int32 [T] of `pages` [n, kv_heads, bytes];
+    a slot that is none (-1) is not written.  qkv stays as it is.  What is held is finite: a NaN becomes zero, an infinity the
+    largest number held."""
+    _geometry(heads, kv_heads, dim, page_size)
+    if not isinstance(qkv, torch.Tensor) or qkv.dim() != 2 or qkv.dtype not in _DT:
+        raise KernelError("qkv: expected rows of bfloat16 or float32")
+    rows, device = qkv.shape[0], qkv.device
+    if cos.dim() != 2 or not 0 < 2 * cos.shape[1] <= dim or cos.shape[0] == 0:
+        raise KernelError(f"rope_write: angles {tuple(cos.shape)} do not fit heads of {dim}")
+    if rows == 0:
+        return q
+    at, n = _pages(pages, kv_heads, dim, page_size)
+    args = (_t(qkv, "qkv", qkv.dtype, (rows, (heads + 2 * kv_heads) * dim), device), _t(positions, "positions", torch.int32, (rows,), device),
+            _t(slots, "slots", torch.int32, (rows,), device), _t(cos, "cos", torch.float32, cos.shape, device),
+            _t(sin, "sin", torch.float32, cos.shape, device), at, _t(q, "q", qkv.dtype, (rows, heads * dim), device))
+    if pages.device != device:
+        raise KernelError(f"pages: on {pages.device}, the others on {device}")
+    _launch("cisr_write4", device, *args, rows, heads, kv_heads, dim, 2 * cos.shape[1], page_size, n, cos.shape[0], int(bool(interleaved)), _DT[qkv.dtype])
+    return q
+
+
+def read(storage, slots, keys, values, kv_heads, dim, page_size):
+    """What token slots `slots` int32 [T] hold at every site of `storage` [sites, n, kv_heads, bytes]: keys and values bfloat16
+    [sites, T, kv_heads, dim], exactly; zeros for a slot that is none."""
+    _geometry(kv_heads, kv_heads, dim, page_size)
+    if not isinstance(storage, torch.Tensor) or storage.dim() != 4 or not 0 < storage.shape[1] < 1 << 31:
+        raise KernelError("storage: expected [sites, n, kv_heads, bytes]")
+    sites, n = storage.shape[:2]
+    rows, device = slots.shape[0], storage.device
+    if rows == 0 or sites == 0:
+        return keys, values
+    at = _t(storage, "storage", torch.uint8, (sites, n, kv_heads, record_bytes(dim, page_size)), None, 16)
+    shape = (sites, rows, kv_heads, dim)
+    _launch("cisr_read4", device, at, _t(slots, "slots", torch.int32, (rows,), device), _t(keys, "keys", torch.bfloat16, shape, device, 16),
+            _t(values, "values", torch.bfloat16, shape, device, 16), sites, rows, kv_heads, dim, page_size, n)
+    return keys, values
+
+
+# -- plans ----------------------------------------------------------------------------------------------------------
+
+COMPUTE_UNITS = 256
+
+
+def launch_of(rows, segments, span, decode_only, heads, kv_heads, dim, dtype):
+    """(form, rows of a task, splits of the keys) for a step of `rows` rows in `segments` segments whose longest has `span` keys.
+    Form 0: a block is 16 items (a row and a query head of the group that shares a key head) whose four waves share the keys; forms 1, 2 and
+    3: four waves of 16, 32 and 64 items that walk the keys side by side."""
+    group = heads // kv_heads
+    steps = -(-span // 32)
+    if decode_only:
+        blocks = rows * kv_heads * -(-group // 16)
+        splits = max(1, min(-(-2 * COMPUTE_UNITS // blocks), steps // 8))
+        return 0, 1, splits
+    form = 1
+    if dtype == torch.bfloat16:
+        for larger in (3, 2):
+            if larger == 3 and padded(dim) > 128:
+                continue
+            if rows * group * kv_heads >= (32 << larger) * COMPUTE_UNITS:
+                form = larger
+                break
+    per_task = max(1, (32 << form) // group)
+    blocks = (-(-rows // per_task) + segments // 2) * kv_heads * -(-per_task * group // (32 << form))
+    splits = max(1, min(COMPUTE_UNITS // max(1, blocks), steps // 8))
+    return form, per_task, splits
+
+
+def weights_form(rows, segments, decode_only, group):
+    """Form 0: four waves with 64 keys each, for the items of few rows; 1 and 2: eight waves share 32 keys (four waves 64) and take the items
+    in turn."""
+    if rows * group <= 64 * segments:
+        return 0
+    return 1 if rows * group < 16384 else 2
+
+
+@dataclass(eq=False)
+class Plan:
+    """A step as the kernels take it: which rows belong to which segment, how many keys each sees, and the launch shapes."""
+    rows: int
+    n_segments: int
+    span: int                          # keys of the longest segment, rounded up or not
+    heads: int
+    kv_heads: int
+    dim: int
+    form: int
+    rows_per_task: int
+    splits: int
+    tasks: torch.Tensor                # int32 [n, 4]: segment (-1: none), first row, rows, keys that the first row sees
+    weights_form: int = 0
+    segments: Optional[torch.Tensor] = None      # int32 [S, 4]: first row, rows, keys before the first row, state slot
+    workspace: Optional[tuple] = None            # (partial results, partial statistics) of split keys
+    slots_below: int = 0               # state slots lie below this number
+
+
+def _whole(numbers, name, least, n=None):
+    out = [operator.index(x) for x in numbers]
+    if n is not None and len(out) != n:
+        raise KernelError(f"cache4.plan: {len(out)} {name} for {n} segments")
+    if any(not least <= x < 1 << 30 for x in out):
+        raise KernelError(f"cache4.plan: {name} out of range")
+    return out
+
+
+def plan(counts, cached, heads, kv_heads, dim, window=None, device="cuda:0", state_slots=None, dtype=torch.bfloat16):
+    """The Plan of a step: segment s brings counts[s] rows (queries) behind cached[s] keys of its request, whose own keys are in the
+    pages too: its row i sees keys 0 .. cached[s] + i (or the last `window` of them).  `state_slots`: where `add_weights` adds a segment's sums,
+    each slot once.  `dtype`: the rows' type."""
+    if kv_heads <= 0 or heads <= 0 or heads % kv_heads or not supported(dim, 8) or dtype not in _DT:
+        raise KernelError(f"cache4.plan: {heads} heads over {kv_heads} of {dim} coordinates in {dtype}")
+    counts = _whole(counts, "counts", 1)
+    cached = _whole(cached, "cached keys", 0, len(counts))
+    window = _window(window)
+    if not counts:
+        raise KernelError("cache4.plan: a step needs a segment")
+    rows, segments = sum(counts), len(counts)
+    longest = max(c + n for c, n in zip(cached, counts))
+    decode_only = rows == segments
+    span = min(longest, window + max(counts)) if window else longest
+    form, per_task, splits = launch_of(rows, segments, span, decode_only, heads, kv_heads, dim, dtype)
+    host = np.zeros((sum(-(-n // per_task) for n in counts), 4), dtype=np.int32)
+    fill_tasks(host, counts, per_task, cached)
+    device = torch.device(device)
+    listed = None
+    if state_slots is not None:
+        slots = _whole(state_slots, "state slots", 0, segments)
+        if len(set(slots)) != segments:
+            raise KernelError("cache4.plan: two segments with one state slot")
+        firsts = np.concatenate(([0], np.cumsum(counts)[:-1]))
+        listed = torch.from_numpy(np.stack([firsts, counts, cached, slots], 1).astype(np.int32)).to(device)
+    made = Plan(rows, segments, longest, heads, kv_heads, dim, form, per_task, splits, torch.from_numpy(host).to(device),
+                weights_form(rows, segments, decode_only, heads // kv_heads), listed, slots_below=1 + max(slots) if state_slots is not None else 0)
+    if splits > 1:
+        made.workspace = (torch.empty(rows * heads * splits * dim, dtype=torch.float32, device=device),
+                          torch.empty(rows * heads * splits * 2, dtype=torch.float32, device=device))
+    return made
+
+
+def _planned(plan, q, tables, heads, kv_heads, dim, page_size, what):
+    _geometry(heads, kv_heads, dim, page_size)
+    if not isinstance(plan, Plan) or (plan.heads, plan.kv_heads, plan.dim) != (heads, kv_heads, dim):
+        raise KernelError(f"{what}: the plan is of other heads")
+    if not isinstance(q, torch.Tensor) or q.dtype not in _DT:
+        raise KernelError("q: expected rows of bfloat16 or float32")
+    if tables.dim() != 2 or tables.shape[0] < plan.n_segments or tables.shape[1] == 0:
+        raise KernelError(f"tables: shape {tuple(tables.shape)} for {plan.n_segments} segments")
+    if q.dtype == torch.float32 and plan.form > 1:
+        raise KernelError(f"{what}: the plan is of rows in bfloat16")
+    device = q.device
+    return device, _t(q, "q", q.dtype, (plan.rows, heads * dim), device, 16), _t(tables, "tables", torch.int32, tables.shape, device)
+
+
+# -- attention ------------------------------------------------------------------------------------------------------
+
+def attention(q, pages, tables, plan, out, heads, kv_heads, dim, page_size, scale, window=None, stats=None):
+    """out [T, heads dim] = softmax(scale q k^T) v of every row over the keys it sees (see `plan`), held in `pages` [n, kv_heads, bytes] of
+    the block tables `tables` int32 [S, W].  Keys behind the table's end, and keys in a page that is none, are not seen; a row that sees
+    none gets zeros.  `stats` float [T, heads]: gets the scores' log-sum-exp in powers of two (-inf for a row that sees none), as
+    `add_weights` takes it.  Rows that the plan does not name are left as they are."""
+    device, qp, tp = _planned(plan, q, tables, heads, kv_heads, dim, page_size, "attention")
+    at, n = _pages(pages, kv_heads, dim, page_size)
+    if pages.device != device or plan.tasks.device != device:
+        raise KernelError(f"attention: pages and plan must be on {device}")
+    op = _t(out, "out", q.dtype, q.shape, device, 8)
+    sp = None if stats is None else _t(stats, "stats", torch.float32, (plan.rows, heads), device)
+    po = pm = None
+    if plan.splits > 1:
+        po, pm = plan.workspace[0].data_ptr(), plan.workspace[1].data_ptr()
+        if plan.workspace[0].numel() < plan.rows * heads * plan.splits * dim or plan.workspace[1].numel() < plan.rows * heads * plan.splits * 2:
+            raise KernelError("attention: the plan's workspace is too small")
+    dt = _DT[q.dtype]
+    _launch(f"cisr_attn4_d{padded(dim)}", device, qp, at, tp, plan.tasks.data_ptr(), op, sp, po, pm, n, plan.tasks.shape[0], plan.rows_per_task, heads,
+            kv_heads, dim, page_size, tables.shape[1], _window(window), _scale(scale), plan.splits, plan.form, dt)
+    if plan.splits > 1:
+        _launch("cisr_merge4", device, po, pm, op, sp, plan.rows * heads, dim, plan.splits, dt)
+    return out
+
+
+def add_weights(q, stats, pages, tables, plan, weights, heads, kv_heads, dim, page_size, scale, window=None):
+    """weights[slot, key head, key] += the key's attention weight, summed over the segment's rows that see it and the query heads
+    that share the key head.  `stats`: what `attention` left for the same rows; weights float [slots, kv_heads, capacity], capacity at least the
+    keys of the longest segment.  The same bits every time: a key's sum has one writer."""
+    device, qp, tp = _planned(plan, q, tables, heads, kv_heads, dim, page_size, "add_weights")
+    at, n = _pages(pages, kv_heads, dim, page_size)
+    if plan.segments is None or plan.segments.device != device or pages.device != device:
+        raise KernelError("add_weights: the plan names no state slots, or is on another device")
+    if weights.dim() != 3 or weights.shape[1] != kv_heads or weights.shape[2] < plan.span or weights.shape[0] < plan.slots_below:
+        raise KernelError(f"weights: shape {tuple(weights.shape)} for {kv_heads} heads of {plan.span} keys in {plan.slots_below} slots")
+    span = min(plan.span, tables.shape[1] * page_size)
+    _launch(f"cisr_weights4_d{padded(dim)}", device, qp, _t(stats, "stats", torch.float32, (plan.rows, heads), device), at, tp, plan.segments.data_ptr(),
+            _t(weights, "weights", torch.float32, weights.shape, device), n, plan.n_segments, span, heads, kv_heads, dim, page_size, tables.shape[1],
+            _window(window), weights.shape[2], weights.shape[0], _scale(scale), plan.weights_form, _DT[q.dtype])
+    return weights
+
+
+# -- a bounded number of keys -----------------------------------------------------------------------------------------
+
+def evict(storage, weights, tables, new_tables, lengths, slots, new_slots, kv_heads, dim, page_size, keep, recent, kept):
+    """Each head of each request keeps, of its first lengths[r] keys, the last `recent` and of the others those with the largest sums
+    of attention weight, `keep` in all (all of them where there are no more); of equal sums the earlier key stays, a NaN counts least.
+    The kept keys and values go, in their order, from the pages of `tables` int32 [R, W] to those of `new_tables` int32 [R, W'] (other
+    pages, W' page_size at least `keep`) at every site of `storage` [sites, n, kv_heads, bytes]; their sums from weights[site][slots[r]]
+    to weights[site][new_slots[r]] (float [n_slots, kv_heads, capacity] a site; it may be the same slot), zeros behind them.
+    kept int32 [sites, R, kv_heads, keep] gets their indices, -1 behind the last.  lengths, slots, new_slots: int32 [R]."""
+    _geometry(kv_heads, kv_heads, dim, page_size)
+    keep, recent = operator.index(keep), operator.index(recent)
+    if keep <= 0 or not 0 <= recent <= keep:
+        raise KernelError(f"evict: {recent} last keys of {keep}")
+    if not isinstance(storage, torch.Tensor) or storage.dim() != 4 or not 0 < storage.shape[1] < 1 << 31:
+        raise KernelError("storage: expected [sites, n, kv_heads, bytes]")
+    sites, n = storage.shape[:2]
+    device, requests = storage.device, lengths.shape[0]
+    if len(weights) != sites or sites == 0:
+        raise KernelError(f"evict: sums of {len(weights)} sites for {sites}")
+    at = _t(storage, "storage", torch.uint8, (sites, n, kv_heads, record_bytes(dim, page_size)), None, 16)
+    n_slots, _, capacity = weights[0].shape
+    if capacity < keep:
+        raise KernelError(f"evict: sums of {capacity} keys, {keep} are kept")
+    sums = [_t(w, "weights", torch.float32, (n_slots, kv_heads, capacity), device) for w in weights]
+    if tables.dim() != 2 or new_tables.dim() != 2 or tables.shape[1] == 0 or new_tables.shape[1] * page_size < keep:
+        raise KernelError(f"evict: tables {tuple(tables.shape)} and {tuple(new_tables.shape)} for {keep} keys")
+    if requests == 0:
+        return kept
+    lp, fp, np_ = (_t(t, name, torch.int32, (requests,), device) for t, name in ((lengths, "lengths"), (slots, "slots"), (new_slots, "new_slots")))
+    _launch("cisr_evict4", device, lp, fp, np_, _t(tables, "tables", torch.int32, (requests, tables.shape[1]), device),
+            _t(new_tables, "new_tables", torch.int32, (requests, new_tables.shape[1]), device), at, (C.c_void_p * sites)(*sums),
+            _t(kept, "kept", torch.int32, (sites, requests, kv_heads, keep), device), sites, n, requests, kv_heads, dim, page_size, tables.shape[1],
+            new_tables.shape[1], keep, recent, capacity, n_slots)
+    return kept

@@ -37,7 +37,8 @@ _libs = {}
 CORE = "kernels"                                   # everything but the matrix-core attention and the measurement kernels
 MEASURE = "measure"                                # kernels that only measure the machine; the engine never loads them
 RECURRENCE = "recurrence"                          # mixers with a state per request: scans, short convolutions, their gates
-OWN_UNITS = (MEASURE, RECURRENCE)                  # units of the source files whose names start with the unit's
+CACHE4 = "cache4"                                  # the cache held in 4 bits: its writes, attention over it, eviction from it
+OWN_UNITS = (MEASURE, RECURRENCE, CACHE4)                  # units of the source files whose names start with the unit's
 ATTENTION_PADS = (32, 64, 96, 128, 160, 192, 224, 256)
 TALKING = "attn_talk"                              # the matrix-core attention whose scores are mixed over the heads (attention_mfma_talk.hip)
 
