@@ -328,30 +328,38 @@ evict4_move(Evict4Args p) {
     }
 }
 
-// Partial results of keys split over blocks: part_o [items][splits][dim], part_ml [items][splits][2] (maximum in powers of two, sum).
+// Partial results of keys in several pieces: part_o [piece][key head][row of the task][head of the group][dim], part_ml likewise [2] (maximum
+// in powers of two, sum).  `merges` [n][4]: first row (negative: none), rows, first piece, pieces.
+struct Merge4Args {
+    const float* part_o; const float* part_ml; const int* merges; void* out; float* stats;
+    int rows_per_task, heads, kv_heads, group, dim;
+};
+
 template <typename T>
 __global__ void __launch_bounds__(256)
-merge4_kernel(const float* part_o, const float* part_ml, T* out, float* stats, int items, int dim, int splits) {
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
-    const int pieces = dim / 2;
-    const long long item = at / pieces;
-    if (item >= items) return;
-    const int d = 2 * (int)(at - item * pieces);
-    const float* ml = part_ml + item * splits * 2;
-    float m = CACHE4_NOTHING;
-    for (int s = 0; s < splits; ++s) m = fmaxf(m, ml[2 * s]);
-    float l = 0.f, a = 0.f, b = 0.f;
-    for (int s = 0; s < splits; ++s) {
-        const float f = exp2f(ml[2 * s] - m);
-        l = fmaf(ml[2 * s + 1], f, l);
-        const float2 v = *(const float2*)(part_o + (item * splits + s) * dim + d);
-        a = fmaf(v.x, f, a);
-        b = fmaf(v.y, f, b);
+merge4_kernel(Merge4Args p) {
+    const int* list = p.merges + 4 * (size_t)blockIdx.x;
+    const int row0 = list[0], rows = list[1], first = list[2], pieces = list[3], halves = p.dim / 2;
+    if (row0 < 0) return;
+    const int at = blockIdx.y * 256 + threadIdx.x, item = at / halves, d = 2 * (at - item * halves);    // (item: row, head)
+    if (item >= rows * p.heads) return;
+    const int r = item / p.heads, h = item - r * p.heads, kvh = h / p.group;
+    const size_t one = ((size_t)kvh * p.rows_per_task + r) * p.group + h - kvh * p.group, step = (size_t)p.heads * p.rows_per_task;
+    float m = CACHE4_NOTHING, l = 0.f, a = 0.f, b = 0.f;
+    for (int s = 0; s < pieces; ++s) {
+        const size_t part = (first + s) * step + one;
+        const float2 ml = *(const float2*)(p.part_ml + 2 * part), v = *(const float2*)(p.part_o + part * p.dim + d);
+        const float top = fmaxf(m, ml.x), f = exp2f(m - top), g = exp2f(ml.x - top);
+        m = top;
+        l = fmaf(ml.y, g, l * f);
+        a = fmaf(v.x, g, a * f);
+        b = fmaf(v.y, g, b * f);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    store_f32(out + item * dim + d, a * inv);
-    store_f32(out + item * dim + d + 1, b * inv);
-    if (stats && d == 0) stats[item] = m + log2f(l);
+    const size_t to = (size_t)(row0 + r) * p.heads + h;
+    if constexpr (sizeof(T) == 4) *(float2*)((float*)p.out + to * p.dim + d) = make_float2(a * inv, b * inv);
+    else *(uint32_t*)((bf16_t*)p.out + to * p.dim + d) = pack_bf16x2(a * inv, b * inv);
+    if (p.stats && d == 0) p.stats[to] = m + log2f(l);
 }
 
 extern "C" {
@@ -408,12 +416,14 @@ int cisr_evict4(const int* lengths, const int* slots, const int* new_slots, cons
     return hipSuccess;
 }
 
-int cisr_merge4(const float* part_o, const float* part_ml, void* out, float* stats, int items, int dim, int splits, int dtype, void* stream) {
-    if (items <= 0 || dim <= 0 || dim % 2 || splits <= 0) return hipErrorInvalidValue;
-    const long long blocks = ((long long)items * (dim / 2) + 255) / 256;
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;
-    if (dtype == DT_BF16) merge4_kernel<<<(int)blocks, 256, 0, (hipStream_t)stream>>>(part_o, part_ml, (bf16_t*)out, stats, items, dim, splits);
-    else merge4_kernel<<<(int)blocks, 256, 0, (hipStream_t)stream>>>(part_o, part_ml, (float*)out, stats, items, dim, splits);
+int cisr_merge4(const float* part_o, const float* part_ml, const int* merges, void* out, float* stats, int n, int rows_per_task, int heads, int kv_heads, int dim, int dtype,
+                void* stream) {
+    if (n <= 0 || rows_per_task <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0 || dim % 2) return hipErrorInvalidValue;
+    const long long blocks = ((long long)rows_per_task * heads * (dim / 2) + 255) / 256;
+    if (blocks > 65535) return hipErrorInvalidValue;
+    Merge4Args p = {part_o, part_ml, merges, out, stats, rows_per_task, heads, kv_heads, heads / kv_heads, dim};
+    if (dtype == DT_BF16) merge4_kernel<bf16_t><<<dim3(n, (int)blocks), 256, 0, (hipStream_t)stream>>>(p);
+    else merge4_kernel<float><<<dim3(n, (int)blocks), 256, 0, (hipStream_t)stream>>>(p);
     return hipGetLastError();
 }
 

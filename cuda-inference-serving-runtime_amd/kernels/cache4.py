@@ -26,7 +26,6 @@ import numpy as np
 import torch
 
 from . import library, ops
-from .attention import fill_tasks
 from .ops import BF16, F32, KernelError
 
 UNIT = library.CACHE4
@@ -59,8 +58,8 @@ def _entry(name):
             "cisr_write4": [p, p, p, p, p, p, p, i, i, i, i, i, i, i, i, i, i, p],
             "cisr_read4": [p, p, p, p, i, i, i, i, i, i, p],
             "cisr_evict4": [p, p, p, p, p, p, p, p, i, i, i, i, i, i, i, i, i, i, i, i, p],
-            "cisr_merge4": [p, p, p, p, i, i, i, i, p],
-            "cisr_attn4": [p, p, p, p, p, p, p, p, ll, i, i, i, i, i, i, i, i, f, i, i, i, p],
+            "cisr_merge4": [p, p, p, p, p, i, i, i, i, i, i, p],
+            "cisr_attn4": [p, p, p, p, p, p, p, p, ll, i, i, i, i, i, i, i, i, f, i, i, p],
             "cisr_weights4": [p, p, p, p, p, p, ll, i, i, i, i, i, i, i, i, i, i, f, i, i, p],
         }[kind]
         fn.restype = C.c_int
@@ -172,30 +171,70 @@ def read(storage, slots, keys, values, kv_heads, dim, page_size):
 # -- plans ----------------------------------------------------------------------------------------------------------
 
 COMPUTE_UNITS = 256
+STEP = 32                  # keys of a step of the kernels
+LEAST_PIECE = 16           # steps of a piece of a row's keys, at least: four for each of the four waves that share them
 
 
-def launch_of(rows, segments, span, decode_only, heads, kv_heads, dim, dtype):
-    """(form, rows of a task, splits of the keys) for a step of `rows` rows in `segments` segments whose longest has `span` keys.
-    Form 0: a block is 16 items (a row and a query head of the group that shares a key head) whose four waves share the keys; forms 1, 2 and
-    3: four waves of 16, 32 and 64 items that walk the keys side by side."""
+def tile_of(form):
+    """Items (a row and a query head of the group that shares a key head) of a block."""
+    return (16, 32, 128)[form]
+
+
+def launch_of(rows, segments, decode_only, heads, kv_heads, dim, dtype):
+    """(form, rows of a task) for a step of `rows` rows in `segments` segments.  Forms 0 and 1: a block is 16 or 32 items whose four
+    waves share the keys; form 2: four waves of 32 items that walk the keys side by side."""
     group = heads // kv_heads
-    steps = -(-span // 32)
-    if decode_only:
-        blocks = rows * kv_heads * -(-group // 16)
-        splits = max(1, min(-(-2 * COMPUTE_UNITS // blocks), steps // 8))
-        return 0, 1, splits
-    form = 1
-    if dtype == torch.bfloat16:
-        for larger in (3, 2):
-            if larger == 3 and padded(dim) > 128:
-                continue
-            if rows * group * kv_heads >= (32 << larger) * COMPUTE_UNITS:
-                form = larger
-                break
-    per_task = max(1, (32 << form) // group)
-    blocks = (-(-rows // per_task) + segments // 2) * kv_heads * -(-per_task * group // (32 << form))
-    splits = max(1, min(COMPUTE_UNITS // max(1, blocks), steps // 8))
-    return form, per_task, splits
+    form = 0
+    if not decode_only and dtype == torch.bfloat16 and padded(dim) <= 128:
+        items = rows * group * kv_heads
+        form = 2 if items >= 128 * COMPUTE_UNITS else 1 if items >= 32 * 2 * COMPUTE_UNITS else 0
+    return form, 1 if decode_only else max(1, tile_of(form) // group)
+
+
+def pieces_for(kv_heads, group, rows_per_task, form):
+    """Pieces that all keys of a step are cut into, at least: blocks for four a compute unit."""
+    return max(1, 4 * COMPUTE_UNITS // (kv_heads * -(-rows_per_task * group // tile_of(form))))
+
+
+def fill_pieces(tasks, merges, counts, cached, rows_per_task, pieces, window):
+    """Writes the tasks of a step (int32 [n, 8], see csrc/cache4_attention.inc) and its merges ([m, 4]: first row, rows, first piece, pieces; -1: none),
+    unused ones at the end; returns how many tasks and merges there are.  Tiles of `rows_per_task` rows of a segment; the keys of long
+    ones are cut so that all pieces are about as long as `pieces` of them would be, the longest first."""
+    counts, cached = np.asarray(counts, dtype=np.int64), np.asarray(cached, dtype=np.int64)
+    tiles = -(-counts // rows_per_task)
+    n = int(tiles.sum())
+    seg = np.repeat(np.arange(len(counts)), tiles)
+    firsts = (np.arange(n) - np.repeat(np.cumsum(tiles) - tiles, tiles)) * rows_per_task
+    row0 = (np.cumsum(counts) - counts)[seg] + firsts
+    rows = np.minimum(rows_per_task, counts[seg] - firsts)
+    sees = cached[seg] + firsts + 1
+    first = np.maximum(0, sees - window) // STEP if window else np.zeros(n, dtype=np.int64)
+    steps = -(-(sees + rows - 1) // STEP) - first
+    each = max(LEAST_PIECE, -(-int(steps.sum()) // pieces))
+    cuts = np.where(2 * steps >= 3 * each, -(-steps // each), 1)
+    share = -(-steps // cuts)
+    cuts = -(-steps // share)
+    of = np.repeat(np.arange(n), cuts)
+    number = np.arange(len(of)) - np.repeat(np.cumsum(cuts) - cuts, cuts)
+    split = cuts > 1
+    piece = np.cumsum(split[of]) - 1
+    made = np.stack([seg[of], row0[of], rows[of], sees[of], first[of] + number * share[of], first[of] + np.minimum((number + 1) * share[of], steps[of]),
+                     np.where(split[of], piece, -1), np.zeros_like(of)], 1)
+    made = made[np.argsort(made[:, 4] - made[:, 5], kind="stable")]
+    tasks[:len(of)] = made
+    tasks[len(of):] = -1
+    m = int(split.sum())
+    if m:
+        begin = np.cumsum(np.where(split, cuts, 0)) - cuts
+        merges[:m] = np.stack([row0, rows, begin, cuts], 1)[split]
+    merges[m:] = -1
+    return len(of), m
+
+
+def most_tasks(rows, segments, rows_per_task, pieces):
+    """(tasks, tiles) that `rows` rows in `segments` segments make at most."""
+    tiles = -(-rows // rows_per_task) + segments
+    return 2 * tiles + pieces, tiles
 
 
 def weights_form(rows, segments, decode_only, group):
@@ -217,8 +256,9 @@ class Plan:
     dim: int
     form: int
     rows_per_task: int
-    splits: int
-    tasks: torch.Tensor                # int32 [n, 4]: segment (-1: none), first row, rows, keys that the first row sees
+    tasks: torch.Tensor                # int32 [n, 8]
+    merges: Optional[torch.Tensor]     # int32 [m, 4], where keys are in several pieces
+    pieces: int = 0                    # pieces that leave partial results
     weights_form: int = 0
     segments: Optional[torch.Tensor] = None      # int32 [S, 4]: first row, rows, keys before the first row, state slot
     workspace: Optional[tuple] = None            # (partial results, partial statistics) of split keys
@@ -248,11 +288,17 @@ def plan(counts, cached, heads, kv_heads, dim, window=None, device="cuda:0", sta
     rows, segments = sum(counts), len(counts)
     longest = max(c + n for c, n in zip(cached, counts))
     decode_only = rows == segments
-    span = min(longest, window + max(counts)) if window else longest
-    form, per_task, splits = launch_of(rows, segments, span, decode_only, heads, kv_heads, dim, dtype)
-    host = np.zeros((sum(-(-n // per_task) for n in counts), 4), dtype=np.int32)
-    fill_tasks(host, counts, per_task, cached)
-    device = torch.device(device)
+    group = heads // kv_heads
+    form, per_task = launch_of(rows, segments, decode_only, heads, kv_heads, dim, dtype)
+    return _plan(counts, cached, heads, kv_heads, dim, window, torch.device(device), state_slots, form, per_task,
+                 pieces_for(kv_heads, group, per_task, form), weights_form(rows, segments, decode_only, group))
+
+
+def _plan(counts, cached, heads, kv_heads, dim, window, device, state_slots, form, per_task, pieces, w_form):
+    rows, segments = sum(counts), len(counts)
+    longest = max(c + n for c, n in zip(cached, counts))
+    tasks, merges = (np.empty((n, k), dtype=np.int32) for n, k in zip(most_tasks(rows, segments, per_task, pieces), (8, 4)))
+    n, m = fill_pieces(tasks, merges, counts, cached, per_task, pieces, window)
     listed = None
     if state_slots is not None:
         slots = _whole(state_slots, "state slots", 0, segments)
@@ -260,11 +306,13 @@ def plan(counts, cached, heads, kv_heads, dim, window=None, device="cuda:0", sta
             raise KernelError("cache4.plan: two segments with one state slot")
         firsts = np.concatenate(([0], np.cumsum(counts)[:-1]))
         listed = torch.from_numpy(np.stack([firsts, counts, cached, slots], 1).astype(np.int32)).to(device)
-    made = Plan(rows, segments, longest, heads, kv_heads, dim, form, per_task, splits, torch.from_numpy(host).to(device),
-                weights_form(rows, segments, decode_only, heads // kv_heads), listed, slots_below=1 + max(slots) if state_slots is not None else 0)
-    if splits > 1:
-        made.workspace = (torch.empty(rows * heads * splits * dim, dtype=torch.float32, device=device),
-                          torch.empty(rows * heads * splits * 2, dtype=torch.float32, device=device))
+    parts = int(tasks[:n, 6].max()) + 1
+    made = Plan(rows, segments, longest, heads, kv_heads, dim, form, per_task, torch.from_numpy(tasks[:n]).to(device),
+                torch.from_numpy(merges[:m]).to(device) if m else None, parts, w_form, listed,
+                slots_below=1 + max(slots) if state_slots is not None else 0)
+    if parts:
+        items = parts * per_task * heads
+        made.workspace = (torch.empty(items * dim, dtype=torch.float32, device=device), torch.empty(items * 2, dtype=torch.float32, device=device))
     return made
 
 
@@ -276,7 +324,7 @@ def _planned(plan, q, tables, heads, kv_heads, dim, page_size, what):
         raise KernelError("q: expected rows of bfloat16 or float32")
     if tables.dim() != 2 or tables.shape[0] < plan.n_segments or tables.shape[1] == 0:
         raise KernelError(f"tables: shape {tuple(tables.shape)} for {plan.n_segments} segments")
-    if q.dtype == torch.float32 and plan.form > 1:
+    if q.dtype == torch.float32 and plan.form > 0:
         raise KernelError(f"{what}: the plan is of rows in bfloat16")
     device = q.device
     return device, _t(q, "q", q.dtype, (plan.rows, heads * dim), device, 16), _t(tables, "tables", torch.int32, tables.shape, device)
@@ -296,15 +344,16 @@ def attention(q, pages, tables, plan, out, heads, kv_heads, dim, page_size, scal
     op = _t(out, "out", q.dtype, q.shape, device, 8)
     sp = None if stats is None else _t(stats, "stats", torch.float32, (plan.rows, heads), device)
     po = pm = None
-    if plan.splits > 1:
+    if plan.pieces:
+        items = plan.pieces * plan.rows_per_task * heads
         po, pm = plan.workspace[0].data_ptr(), plan.workspace[1].data_ptr()
-        if plan.workspace[0].numel() < plan.rows * heads * plan.splits * dim or plan.workspace[1].numel() < plan.rows * heads * plan.splits * 2:
+        if plan.workspace[0].numel() < items * dim or plan.workspace[1].numel() < items * 2:
             raise KernelError("attention: the plan's workspace is too small")
     dt = _DT[q.dtype]
     _launch(f"cisr_attn4_d{padded(dim)}", device, qp, at, tp, plan.tasks.data_ptr(), op, sp, po, pm, n, plan.tasks.shape[0], plan.rows_per_task, heads,
-            kv_heads, dim, page_size, tables.shape[1], _window(window), _scale(scale), plan.splits, plan.form, dt)
-    if plan.splits > 1:
-        _launch("cisr_merge4", device, po, pm, op, sp, plan.rows * heads, dim, plan.splits, dt)
+            kv_heads, dim, page_size, tables.shape[1], _window(window), _scale(scale), plan.form, dt)
+    if plan.merges is not None:
+        _launch("cisr_merge4", device, po, pm, plan.merges.data_ptr(), op, sp, plan.merges.shape[0], plan.rows_per_task, heads, kv_heads, dim, dt)
     return out
 
 

@@ -127,7 +127,7 @@ def check_step(counts, cached, heads, kv, dim, P, kind, window=0, weights=False,
     S, rows = len(counts), sum(counts)
     plan = c.plan(counts, cached, heads, kv, dim, window=window, dtype=dtype, state_slots=[S - s for s in range(S)] if weights else None)
     if force is not None:
-        plan = forced(c, plan, counts, cached, *force)
+        plan = forced(c, plan, counts, cached, *force, window)
     out = torch.full((rows, heads * dim), math.nan, dtype=dtype, device=GPU)
     stats = torch.empty(rows, heads, device=GPU) if weights else None
     gq, gp, gt = q.to(GPU), pages.to(GPU), tables.to(GPU)
@@ -161,18 +161,11 @@ def check_step(counts, cached, heads, kv, dim, P, kind, window=0, weights=False,
         assert ((sums - expected_sums).abs() <= room * 1.01).all()
 
 
-def forced(c, plan, counts, cached, form, splits):
-    """The plan with another form and another number of splits."""
-    import numpy as np
+def forced(c, plan, counts, cached, form, pieces, window):
+    """The plan with another form and another number of pieces."""
     group = plan.heads // plan.kv_heads
-    per_task = 1 if form == 0 else max(1, (32 << form) // group)
-    host = np.zeros((sum(-(-n // per_task) for n in counts), 4), dtype=np.int32)
-    c.fill_tasks(host, counts, per_task, cached)
-    plan.form, plan.rows_per_task, plan.splits = form, per_task, splits
-    plan.tasks = torch.from_numpy(host).to(GPU)
-    items = plan.rows * plan.heads * splits
-    plan.workspace = (torch.empty(items * plan.dim, device=GPU), torch.empty(items * 2, device=GPU))
-    return plan
+    per_task = max(1, c.tile_of(form) // group)
+    return c._plan(counts, cached, plan.heads, plan.kv_heads, plan.dim, window, torch.device(GPU), None, form, per_task, pieces, plan.weights_form)
 
 
 HEADS = [(9, 3, 64), (4, 4, 64), (8, 2, 128), (6, 2, 96), (5, 5, 16), (4, 1, 80), (16, 2, 256), (3, 1, 20), (2, 1, 160), (2, 2, 192), (3, 1, 224), (40, 1, 64), (34, 2, 32)]
@@ -197,12 +190,13 @@ def test_windows_and_pages(P, window, counts, cached):
     check_step(counts, cached, 6, 2, 64, P, "bf16", window=window, weights=True)
 
 
-@pytest.mark.parametrize("splits", [1, 3, 9])
-@pytest.mark.parametrize("form,heads,kv,dim,kind", [(form, *h, kind) for form in range(4) for h in ((9, 3, 64), (8, 2, 128), (2, 1, 256), (6, 2, 96))
-                                                    for kind in TYPES if not (form > 1 and kind == "f32") and not (form == 3 and h[2] > 128)])
-@pytest.mark.parametrize("window", [0, 50])
-def test_forms_and_splits(form, splits, heads, kv, dim, window, kind):
-    check_step([90, 1, 33], [10, 70, 200], heads, kv, dim, 16, kind, window=window, force=(form, splits))
+@pytest.mark.parametrize("pieces", [1, 20])
+@pytest.mark.parametrize("form,heads,kv,dim,kind", [(form, *h, kind) for form in range(3) for h in ((9, 3, 64), (8, 2, 128), (2, 1, 256), (6, 2, 96))
+                                                    for kind in TYPES if form == 0 or (kind == "bf16" and h[2] <= 128)])
+@pytest.mark.parametrize("window", [0, 50, 400])
+def test_forms_and_pieces(form, pieces, heads, kv, dim, window, kind, monkeypatch):
+    monkeypatch.setattr(cache4(), "LEAST_PIECE", 2)
+    check_step([90, 1, 33], [10, 70, 500], heads, kv, dim, 16, kind, window=window, force=(form, pieces))
 
 
 @pytest.mark.parametrize("weights_form", [0, 1, 2])
