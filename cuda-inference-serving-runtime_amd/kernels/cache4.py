@@ -16,10 +16,11 @@ or float32.
 time: two streams need two plans.
 The reference has nothing of this kind (its cache is float32 and keeps every key, runtime/cache.py:9-118).
 """
-import contextlib
 import ctypes as C
+import functools
+import math
 import operator
-from dataclasses import dataclass, field
+from dataclasses import dataclass
 from typing import Optional
 
 import numpy as np
@@ -60,67 +61,84 @@ def _entry(name):
             "cisr_evict4": [p, p, p, p, p, p, p, p, i, i, i, i, i, i, i, i, i, i, i, i, p],
             "cisr_merge4": [p, p, p, p, p, i, i, i, i, i, i, p],
             "cisr_attn4": [p, p, p, p, p, p, p, p, ll, i, i, i, i, i, i, i, i, f, i, i, p],
-            "cisr_weights4": [p, p, p, p, p, p, ll, i, i, i, i, i, i, i, i, i, i, f, i, i, p],
+            "cisr_weights4": [p, p, p, p, p, p, p, ll, i, i, i, i, i, i, i, i, i, i, f, i, i, i, p],
         }[kind]
         fn.restype = C.c_int
         _entries[name] = fn
     return fn
 
 
-def _t(t, name, dtype, shape, device=None, align=1):
-    """The address of a contiguous GPU tensor of that type and shape (on `device`, on so many bytes)."""
+def _t(t, name, dtype, shape, index, align=1):
+    """The address of a contiguous tensor of that type and shape on GPU `index` (on so many bytes).  (Asked eight times a call: what is right costs
+    half a microsecond, what is wrong is found out afterwards.)"""
+    try:
+        if t.dtype is dtype and t.shape == shape and t.is_contiguous() and t.get_device() == index:
+            at = t.data_ptr()
+            if at % align == 0:
+                return at
+    except AttributeError:
+        pass
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise KernelError(f"{name}: expected a GPU tensor")
     if t.dtype != dtype:
         raise KernelError(f"{name}: dtype {t.dtype}, expected {dtype}")
-    if t.shape != shape:
+    if tuple(t.shape) != tuple(shape):
         raise KernelError(f"{name}: shape {tuple(t.shape)}, expected {tuple(shape)}")
     if not t.is_contiguous():
         raise KernelError(f"{name}: tensor must be contiguous")
-    if device is not None and t.device != device:
-        raise KernelError(f"{name}: on {t.device}, the others on {device}")
-    at = t.data_ptr()
-    if at % align:
-        raise KernelError(f"{name}: must lie on {align} bytes")
-    return at
+    if t.get_device() != index:
+        raise KernelError(f"{name}: on {t.device}, the others on cuda:{index}")
+    raise KernelError(f"{name}: must lie on {align} bytes")
 
 
-def _geometry(heads, kv_heads, dim, page_size):
+@functools.lru_cache(maxsize=256)
+def _record(heads, kv_heads, dim, page_size):
+    """Bytes of a head's page, for sizes that the kernels take."""
     if not supported(dim, page_size):
         raise KernelError(f"cache4: heads of {dim} in pages of {page_size}: an even size up to {MAX_HEAD}, a power of two from 8 on")
     if kv_heads <= 0 or heads <= 0 or heads % kv_heads:
         raise KernelError(f"cache4: {heads} query heads are not a multiple of {kv_heads} key/value heads")
+    return record_bytes(dim, page_size)
 
 
-def _pages(pages, kv_heads, dim, page_size, name="pages"):
-    """(address, pages) of one site's pages [n, kv_heads, bytes]."""
-    if not isinstance(pages, torch.Tensor) or pages.dim() != 3 or not 0 < pages.shape[0] < 1 << 31:
-        raise KernelError(f"{name}: expected pages of one site, [n, kv_heads, bytes]")
-    return _t(pages, name, torch.uint8, (pages.shape[0], kv_heads, record_bytes(dim, page_size)), None, 16), pages.shape[0]
+def _gpu_of(t, name, dims):
+    """The index of the GPU that tensor `t`, of so many dimensions, is on."""
+    if not isinstance(t, torch.Tensor) or t.dim() != dims or not t.is_cuda:
+        raise KernelError(f"{name}: expected a GPU tensor of {dims} dimensions")
+    return t.get_device()
 
 
-def _on(device):
-    """The tensors' device as the current one, for the launch (their stream is that device's current one)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+def _pool(pages, what):
+    """How many pages a pool has (page numbers are 32-bit)."""
+    n = pages.shape[-3]
+    if not 0 < n < 1 << 31:
+        raise KernelError(f"{what}: a pool of {n} pages")
+    return n
 
 
-def _launch(name, device, *args):
-    with _on(device):
-        code = _entry(name)(*args, ops._stream())
+def _launch(name, index, *args):
+    """Runs an entry point on the current stream of GPU `index`."""
+    fn = _entries.get(name) or _entry(name)
+    if ops._raw_stream is not None and ops._current_device is not None and ops._current_device() == index:
+        code = fn(*args, ops._raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, ops._stream())
     if code:
         raise KernelError(f"{name}: HIP error {code}")
 
 
 def _scale(scale):
-    scale = float(scale)
-    if not 0.0 < scale < float("inf"):
+    if not 0.0 < scale < math.inf:
         raise KernelError(f"cache4: the score scale must be positive, not {scale}")
-    return scale
+    return float(scale)
 
 
 def _window(window):
-    window = operator.index(window or 0)
-    if not 0 <= window < 1 << 31:
+    if not window:
+        return 0
+    window = operator.index(window)
+    if not 0 < window < 1 << 30:
         raise KernelError(f"cache4: a window of {window} keys")
     return window
 
@@ -133,38 +151,34 @@ def rope_write(qkv, positions, slots, cos, sin, pages, q, heads, kv_heads, dim, 
     the queries into q [T, heads dim] and holds keys and values in the token slots `slots` int32 [T] of `pages` [n, kv_heads, bytes];
     a slot that is none (-1) is not written.  qkv stays as it is.  What is held is finite: a NaN becomes zero, an infinity the
     largest number held."""
-    _geometry(heads, kv_heads, dim, page_size)
-    if not isinstance(qkv, torch.Tensor) or qkv.dim() != 2 or qkv.dtype not in _DT:
+    record = _record(heads, kv_heads, dim, page_size)
+    index = _gpu_of(qkv, "qkv", 2)
+    dtype, rows = qkv.dtype, qkv.shape[0]
+    if dtype not in _DT:
         raise KernelError("qkv: expected rows of bfloat16 or float32")
-    rows, device = qkv.shape[0], qkv.device
     if cos.dim() != 2 or not 0 < 2 * cos.shape[1] <= dim or cos.shape[0] == 0:
         raise KernelError(f"rope_write: angles {tuple(cos.shape)} do not fit heads of {dim}")
-    if rows == 0:
-        return q
-    at, n = _pages(pages, kv_heads, dim, page_size)
-    args = (_t(qkv, "qkv", qkv.dtype, (rows, (heads + 2 * kv_heads) * dim), device), _t(positions, "positions", torch.int32, (rows,), device),
-            _t(slots, "slots", torch.int32, (rows,), device), _t(cos, "cos", torch.float32, cos.shape, device),
-            _t(sin, "sin", torch.float32, cos.shape, device), at, _t(q, "q", qkv.dtype, (rows, heads * dim), device))
-    if pages.device != device:
-        raise KernelError(f"pages: on {pages.device}, the others on {device}")
-    _launch("cisr_write4", device, *args, rows, heads, kv_heads, dim, 2 * cos.shape[1], page_size, n, cos.shape[0], int(bool(interleaved)), _DT[qkv.dtype])
+    if _gpu_of(pages, "pages", 3) != index:
+        raise KernelError("rope_write: pages and rows on different GPUs")
+    n, table = _pool(pages, "rope_write"), cos.shape
+    if rows:
+        _launch("cisr_write4", index, _t(qkv, "qkv", dtype, (rows, (heads + 2 * kv_heads) * dim), index), _t(positions, "positions", torch.int32, (rows,), index),
+                _t(slots, "slots", torch.int32, (rows,), index), _t(cos, "cos", torch.float32, table, index), _t(sin, "sin", torch.float32, table, index),
+                _t(pages, "pages", torch.uint8, (n, kv_heads, record), index, 16), _t(q, "q", dtype, (rows, heads * dim), index), rows, heads, kv_heads, dim,
+                2 * table[1], page_size, n, table[0], int(bool(interleaved)), _DT[dtype])
     return q
 
 
 def read(storage, slots, keys, values, kv_heads, dim, page_size):
     """What token slots `slots` int32 [T] hold at every site of `storage` [sites, n, kv_heads, bytes]: keys and values bfloat16
     [sites, T, kv_heads, dim], exactly; zeros for a slot that is none."""
-    _geometry(kv_heads, kv_heads, dim, page_size)
-    if not isinstance(storage, torch.Tensor) or storage.dim() != 4 or not 0 < storage.shape[1] < 1 << 31:
-        raise KernelError("storage: expected [sites, n, kv_heads, bytes]")
-    sites, n = storage.shape[:2]
-    rows, device = slots.shape[0], storage.device
-    if rows == 0 or sites == 0:
-        return keys, values
-    at = _t(storage, "storage", torch.uint8, (sites, n, kv_heads, record_bytes(dim, page_size)), None, 16)
+    record = _record(kv_heads, kv_heads, dim, page_size)
+    index = _gpu_of(storage, "storage", 4)
+    n, sites, rows = _pool(storage, "read"), storage.shape[0], slots.shape[0]
     shape = (sites, rows, kv_heads, dim)
-    _launch("cisr_read4", device, at, _t(slots, "slots", torch.int32, (rows,), device), _t(keys, "keys", torch.bfloat16, shape, device, 16),
-            _t(values, "values", torch.bfloat16, shape, device, 16), sites, rows, kv_heads, dim, page_size, n)
+    if rows and sites:
+        _launch("cisr_read4", index, _t(storage, "storage", torch.uint8, (sites, n, kv_heads, record), index, 16), _t(slots, "slots", torch.int32, (rows,), index),
+                _t(keys, "keys", torch.bfloat16, shape, index, 16), _t(values, "values", torch.bfloat16, shape, index, 16), sites, rows, kv_heads, dim, page_size, n)
     return keys, values
 
 
@@ -191,9 +205,9 @@ def launch_of(rows, segments, decode_only, heads, kv_heads, dim, dtype):
     return form, 1 if decode_only else max(1, tile_of(form) // group)
 
 
-def pieces_for(kv_heads, group, rows_per_task, form):
-    """Pieces that all keys of a step are cut into, at least: blocks for four a compute unit."""
-    return max(1, 4 * COMPUTE_UNITS // (kv_heads * -(-rows_per_task * group // tile_of(form))))
+def pieces_for(kv_heads, group, rows_per_task, form, decode_only):
+    """Pieces that all keys of a step are cut into, at least: blocks for four a compute unit, for two where rows of a prompt make many tiles anyway."""
+    return max(1, (4 if decode_only else 2) * COMPUTE_UNITS // (kv_heads * -(-rows_per_task * group // tile_of(form))))
 
 
 def fill_pieces(tasks, merges, counts, cached, rows_per_task, pieces, window):
@@ -237,12 +251,14 @@ def most_tasks(rows, segments, rows_per_task, pieces):
     return 2 * tiles + pieces, tiles
 
 
-def weights_form(rows, segments, decode_only, group):
-    """Form 0: four waves with 64 keys each, for the items of few rows; 1 and 2: eight waves share 32 keys (four waves 64) and take the items
-    in turn."""
-    if rows * group <= 64 * segments:
+def shares_of(rows, segments, span, group, kv_heads):
+    """Into how many shares the items (a row and a head of the group) of a segment are cut where the keys' attention weights are summed; 0: few
+    items, a wave has them all and walks the keys.  Blocks (128 keys and a share) for two a compute unit, 256 items a share at least."""
+    items = -(-rows * group // segments)
+    if items <= 64:
         return 0
-    return 1 if rows * group < 16384 else 2
+    blocks = -(-span // 128) * kv_heads * segments
+    return max(1, min(2 * COMPUTE_UNITS // blocks, items // 256, 65535 // segments))
 
 
 @dataclass(eq=False)
@@ -258,11 +274,26 @@ class Plan:
     rows_per_task: int
     tasks: torch.Tensor                # int32 [n, 8]
     merges: Optional[torch.Tensor]     # int32 [m, 4], where keys are in several pieces
-    pieces: int = 0                    # pieces that leave partial results
-    weights_form: int = 0
+    pieces: int = 0                    # pieces that leave partial results, at most
     segments: Optional[torch.Tensor] = None      # int32 [S, 4]: first row, rows, keys before the first row, state slot
-    workspace: Optional[tuple] = None            # (partial results, partial statistics) of split keys
     slots_below: int = 0               # state slots lie below this number
+    shares: int = 0                    # see shares_of
+    room: Optional[torch.Tensor] = None          # floats for partial results: of `attention` room_of, of `add_weights` parts_of (one after the other)
+
+    def __post_init__(self):
+        self.index = self.tasks.get_device()
+        if self.room is None and max(self.room_of, self.parts_of):
+            self.room = torch.empty(max(self.room_of, self.parts_of), dtype=torch.float32, device=self.tasks.device)
+        if self.room is not None and self.room.numel() < max(self.room_of, self.parts_of):
+            raise KernelError("cache4: a plan's workspace is too small")
+
+    @property
+    def room_of(self):
+        return self.pieces * self.rows_per_task * self.heads * (self.dim + 2)
+
+    @property
+    def parts_of(self):
+        return self.shares * self.n_segments * self.kv_heads * self.span if self.shares > 1 else 0
 
 
 def _whole(numbers, name, least, n=None):
@@ -291,10 +322,10 @@ def plan(counts, cached, heads, kv_heads, dim, window=None, device="cuda:0", sta
     group = heads // kv_heads
     form, per_task = launch_of(rows, segments, decode_only, heads, kv_heads, dim, dtype)
     return _plan(counts, cached, heads, kv_heads, dim, window, torch.device(device), state_slots, form, per_task,
-                 pieces_for(kv_heads, group, per_task, form), weights_form(rows, segments, decode_only, group))
+                 pieces_for(kv_heads, group, per_task, form, decode_only))
 
 
-def _plan(counts, cached, heads, kv_heads, dim, window, device, state_slots, form, per_task, pieces, w_form):
+def _plan(counts, cached, heads, kv_heads, dim, window, device, state_slots, form, per_task, pieces):
     rows, segments = sum(counts), len(counts)
     longest = max(c + n for c, n in zip(cached, counts))
     tasks, merges = (np.empty((n, k), dtype=np.int32) for n, k in zip(most_tasks(rows, segments, per_task, pieces), (8, 4)))
@@ -307,27 +338,24 @@ def _plan(counts, cached, heads, kv_heads, dim, window, device, state_slots, for
         firsts = np.concatenate(([0], np.cumsum(counts)[:-1]))
         listed = torch.from_numpy(np.stack([firsts, counts, cached, slots], 1).astype(np.int32)).to(device)
     parts = int(tasks[:n, 6].max()) + 1
-    made = Plan(rows, segments, longest, heads, kv_heads, dim, form, per_task, torch.from_numpy(tasks[:n]).to(device),
-                torch.from_numpy(merges[:m]).to(device) if m else None, parts, w_form, listed,
-                slots_below=1 + max(slots) if state_slots is not None else 0)
-    if parts:
-        items = parts * per_task * heads
-        made.workspace = (torch.empty(items * dim, dtype=torch.float32, device=device), torch.empty(items * 2, dtype=torch.float32, device=device))
-    return made
+    return Plan(rows, segments, longest, heads, kv_heads, dim, form, per_task, torch.from_numpy(tasks[:n]).to(device),
+                torch.from_numpy(merges[:m]).to(device) if m else None, parts, listed, 0 if listed is None else 1 + max(slots),
+                0 if listed is None else shares_of(rows, segments, longest, heads // kv_heads, kv_heads))
 
 
-def _planned(plan, q, tables, heads, kv_heads, dim, page_size, what):
-    _geometry(heads, kv_heads, dim, page_size)
+def _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, what):
+    """(GPU, bytes of a head's page, pages) of a planned step, checked against its plan."""
+    record = _record(heads, kv_heads, dim, page_size)
+    index = _gpu_of(q, "q", 2)
     if not isinstance(plan, Plan) or (plan.heads, plan.kv_heads, plan.dim) != (heads, kv_heads, dim):
         raise KernelError(f"{what}: the plan is of other heads")
-    if not isinstance(q, torch.Tensor) or q.dtype not in _DT:
-        raise KernelError("q: expected rows of bfloat16 or float32")
-    if tables.dim() != 2 or tables.shape[0] < plan.n_segments or tables.shape[1] == 0:
+    if q.dtype not in _DT or (plan.form > 0 and q.dtype is not torch.bfloat16):
+        raise KernelError(f"{what}: rows in {q.dtype}: bfloat16 or float32, as planned")
+    if plan.index != index or _gpu_of(pages, "pages", 3) != index:
+        raise KernelError(f"{what}: rows, pages and plan on different GPUs")
+    if tables.dim() != 2 or tables.shape[0] < plan.n_segments or not 0 < tables.shape[1] * page_size < 1 << 31:
         raise KernelError(f"tables: shape {tuple(tables.shape)} for {plan.n_segments} segments")
-    if q.dtype == torch.float32 and plan.form > 0:
-        raise KernelError(f"{what}: the plan is of rows in bfloat16")
-    device = q.device
-    return device, _t(q, "q", q.dtype, (plan.rows, heads * dim), device, 16), _t(tables, "tables", torch.int32, tables.shape, device)
+    return index, record, _pool(pages, what)
 
 
 # -- attention ------------------------------------------------------------------------------------------------------
@@ -337,23 +365,20 @@ def attention(q, pages, tables, plan, out, heads, kv_heads, dim, page_size, scal
     the block tables `tables` int32 [S, W].  Keys behind the table's end, and keys in a page that is none, are not seen; a row that sees
     none gets zeros.  `stats` float [T, heads]: gets the scores' log-sum-exp in powers of two (-inf for a row that sees none), as
     `add_weights` takes it.  Rows that the plan does not name are left as they are."""
-    device, qp, tp = _planned(plan, q, tables, heads, kv_heads, dim, page_size, "attention")
-    at, n = _pages(pages, kv_heads, dim, page_size)
-    if pages.device != device or plan.tasks.device != device:
-        raise KernelError(f"attention: pages and plan must be on {device}")
-    op = _t(out, "out", q.dtype, q.shape, device, 8)
-    sp = None if stats is None else _t(stats, "stats", torch.float32, (plan.rows, heads), device)
+    index, record, n = _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, "attention")
+    dtype, rows = q.dtype, plan.rows
+    op = _t(out, "out", dtype, (rows, heads * dim), index, 8)
+    sp = None if stats is None else _t(stats, "stats", torch.float32, (rows, heads), index)
     po = pm = None
     if plan.pieces:
-        items = plan.pieces * plan.rows_per_task * heads
-        po, pm = plan.workspace[0].data_ptr(), plan.workspace[1].data_ptr()
-        if plan.workspace[0].numel() < items * dim or plan.workspace[1].numel() < items * 2:
-            raise KernelError("attention: the plan's workspace is too small")
-    dt = _DT[q.dtype]
-    _launch(f"cisr_attn4_d{padded(dim)}", device, qp, at, tp, plan.tasks.data_ptr(), op, sp, po, pm, n, plan.tasks.shape[0], plan.rows_per_task, heads,
+        po = plan.room.data_ptr()
+        pm = po + 4 * plan.pieces * plan.rows_per_task * heads * dim
+    dt = _DT[dtype]
+    _launch(f"cisr_attn4_d{padded(dim)}", index, _t(q, "q", dtype, (rows, heads * dim), index, 16), _t(pages, "pages", torch.uint8, (n, kv_heads, record), index, 16),
+            _t(tables, "tables", torch.int32, tables.shape, index), plan.tasks.data_ptr(), op, sp, po, pm, n, plan.tasks.shape[0], plan.rows_per_task, heads,
             kv_heads, dim, page_size, tables.shape[1], _window(window), _scale(scale), plan.form, dt)
     if plan.merges is not None:
-        _launch("cisr_merge4", device, po, pm, plan.merges.data_ptr(), op, sp, plan.merges.shape[0], plan.rows_per_task, heads, kv_heads, dim, dt)
+        _launch("cisr_merge4", index, po, pm, plan.merges.data_ptr(), op, sp, plan.merges.shape[0], plan.rows_per_task, heads, kv_heads, dim, dt)
     return out
 
 
@@ -361,16 +386,18 @@ def add_weights(q, stats, pages, tables, plan, weights, heads, kv_heads, dim, pa
     """weights[slot, key head, key] += the key's attention weight, summed over the segment's rows that see it and the query heads
     that share the key head.  `stats`: what `attention` left for the same rows; weights float [slots, kv_heads, capacity], capacity at least the
     keys of the longest segment.  The same bits every time: a key's sum has one writer."""
-    device, qp, tp = _planned(plan, q, tables, heads, kv_heads, dim, page_size, "add_weights")
-    at, n = _pages(pages, kv_heads, dim, page_size)
-    if plan.segments is None or plan.segments.device != device or pages.device != device:
-        raise KernelError("add_weights: the plan names no state slots, or is on another device")
-    if weights.dim() != 3 or weights.shape[1] != kv_heads or weights.shape[2] < plan.span or weights.shape[0] < plan.slots_below:
+    index, record, n = _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, "add_weights")
+    if plan.segments is None:
+        raise KernelError("add_weights: the plan names no state slots")
+    if _gpu_of(weights, "weights", 3) != index or weights.shape[1] != kv_heads or weights.shape[2] < plan.span or weights.shape[0] < plan.slots_below:
         raise KernelError(f"weights: shape {tuple(weights.shape)} for {kv_heads} heads of {plan.span} keys in {plan.slots_below} slots")
-    span = min(plan.span, tables.shape[1] * page_size)
-    _launch(f"cisr_weights4_d{padded(dim)}", device, qp, _t(stats, "stats", torch.float32, (plan.rows, heads), device), at, tp, plan.segments.data_ptr(),
-            _t(weights, "weights", torch.float32, weights.shape, device), n, plan.n_segments, span, heads, kv_heads, dim, page_size, tables.shape[1],
-            _window(window), weights.shape[2], weights.shape[0], _scale(scale), plan.weights_form, _DT[q.dtype])
+    blocks = max(1, min(-(-plan.span // (4 * STEP)), -(-4 * COMPUTE_UNITS // (kv_heads * plan.n_segments))))      # (of four waves: four a compute unit)
+    slots, _, capacity = weights.shape
+    _launch(f"cisr_weights4_d{padded(dim)}", index, _t(q, "q", q.dtype, (plan.rows, heads * dim), index, 16),
+            _t(stats, "stats", torch.float32, (plan.rows, heads), index), _t(pages, "pages", torch.uint8, (n, kv_heads, record), index, 16),
+            _t(tables, "tables", torch.int32, tables.shape, index), plan.segments.data_ptr(), _t(weights, "weights", torch.float32, weights.shape, index),
+            None if plan.shares < 2 else plan.room.data_ptr(), n, plan.n_segments, plan.span, heads, kv_heads, dim, page_size, tables.shape[1], _window(window),
+            capacity, slots, _scale(scale), plan.shares, blocks, _DT[q.dtype])
     return weights
 
 
@@ -383,28 +410,26 @@ def evict(storage, weights, tables, new_tables, lengths, slots, new_slots, kv_he
     pages, W' page_size at least `keep`) at every site of `storage` [sites, n, kv_heads, bytes]; their sums from weights[site][slots[r]]
     to weights[site][new_slots[r]] (float [n_slots, kv_heads, capacity] a site; it may be the same slot), zeros behind them.
     kept int32 [sites, R, kv_heads, keep] gets their indices, -1 behind the last.  lengths, slots, new_slots: int32 [R]."""
-    _geometry(kv_heads, kv_heads, dim, page_size)
+    record = _record(kv_heads, kv_heads, dim, page_size)
     keep, recent = operator.index(keep), operator.index(recent)
-    if keep <= 0 or not 0 <= recent <= keep:
+    if not 0 < keep < 1 << 30 or not 0 <= recent <= keep:
         raise KernelError(f"evict: {recent} last keys of {keep}")
-    if not isinstance(storage, torch.Tensor) or storage.dim() != 4 or not 0 < storage.shape[1] < 1 << 31:
-        raise KernelError("storage: expected [sites, n, kv_heads, bytes]")
-    sites, n = storage.shape[:2]
-    device, requests = storage.device, lengths.shape[0]
+    index = _gpu_of(storage, "storage", 4)
+    n, sites, requests = _pool(storage, "evict"), storage.shape[0], lengths.shape[0]
     if len(weights) != sites or sites == 0:
         raise KernelError(f"evict: sums of {len(weights)} sites for {sites}")
-    at = _t(storage, "storage", torch.uint8, (sites, n, kv_heads, record_bytes(dim, page_size)), None, 16)
+    _gpu_of(weights[0], "weights", 3)
     n_slots, _, capacity = weights[0].shape
     if capacity < keep:
         raise KernelError(f"evict: sums of {capacity} keys, {keep} are kept")
-    sums = [_t(w, "weights", torch.float32, (n_slots, kv_heads, capacity), device) for w in weights]
     if tables.dim() != 2 or new_tables.dim() != 2 or tables.shape[1] == 0 or new_tables.shape[1] * page_size < keep:
         raise KernelError(f"evict: tables {tuple(tables.shape)} and {tuple(new_tables.shape)} for {keep} keys")
-    if requests == 0:
-        return kept
-    lp, fp, np_ = (_t(t, name, torch.int32, (requests,), device) for t, name in ((lengths, "lengths"), (slots, "slots"), (new_slots, "new_slots")))
-    _launch("cisr_evict4", device, lp, fp, np_, _t(tables, "tables", torch.int32, (requests, tables.shape[1]), device),
-            _t(new_tables, "new_tables", torch.int32, (requests, new_tables.shape[1]), device), at, (C.c_void_p * sites)(*sums),
-            _t(kept, "kept", torch.int32, (sites, requests, kv_heads, keep), device), sites, n, requests, kv_heads, dim, page_size, tables.shape[1],
-            new_tables.shape[1], keep, recent, capacity, n_slots)
+    sums = [_t(w, "weights", torch.float32, (n_slots, kv_heads, capacity), index) for w in weights]
+    if requests:
+        _launch("cisr_evict4", index, _t(lengths, "lengths", torch.int32, (requests,), index), _t(slots, "slots", torch.int32, (requests,), index),
+                _t(new_slots, "new_slots", torch.int32, (requests,), index), _t(tables, "tables", torch.int32, (requests, tables.shape[1]), index),
+                _t(new_tables, "new_tables", torch.int32, (requests, new_tables.shape[1]), index),
+                _t(storage, "storage", torch.uint8, (sites, n, kv_heads, record), index, 16), (C.c_void_p * sites)(*sums),
+                _t(kept, "kept", torch.int32, (sites, requests, kv_heads, keep), index), sites, n, requests, kv_heads, dim, page_size, tables.shape[1],
+                new_tables.shape[1], keep, recent, capacity, n_slots)
     return kept

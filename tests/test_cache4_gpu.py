@@ -165,7 +165,7 @@ def forced(c, plan, counts, cached, form, pieces, window):
     """The plan with another form and another number of pieces."""
     group = plan.heads // plan.kv_heads
     per_task = max(1, c.tile_of(form) // group)
-    return c._plan(counts, cached, plan.heads, plan.kv_heads, plan.dim, window, torch.device(GPU), None, form, per_task, pieces, plan.weights_form)
+    return c._plan(counts, cached, plan.heads, plan.kv_heads, plan.dim, window, torch.device(GPU), None, form, per_task, pieces)
 
 
 HEADS = [(9, 3, 64), (4, 4, 64), (8, 2, 128), (6, 2, 96), (5, 5, 16), (4, 1, 80), (16, 2, 256), (3, 1, 20), (2, 1, 160), (2, 2, 192), (3, 1, 224), (40, 1, 64), (34, 2, 32)]
@@ -199,14 +199,13 @@ def test_forms_and_pieces(form, pieces, heads, kv, dim, window, kind, monkeypatc
     check_step([90, 1, 33], [10, 70, 500], heads, kv, dim, 16, kind, window=window, force=(form, pieces))
 
 
-@pytest.mark.parametrize("weights_form", [0, 1, 2])
+@pytest.mark.parametrize("shares", [0, 1, 2, 5])
 @pytest.mark.parametrize("window", [0, 30])
-def test_forms_of_the_sums(weights_form, window, monkeypatch):
-    c = cache4()
-    monkeypatch.setattr(c, "weights_form", lambda *a: weights_form)
-    if weights_form == 0:
-        check_step([3, 1, 2], [40, 0, 300], 8, 2, 128, 16, "bf16", window=window, weights=True)
-    check_step([150, 1, 40], [10, 70, 200], 9, 3, 64, 16, "bf16", window=window, weights=True)
+@pytest.mark.parametrize("heads,kv,dim,kind", [(8, 2, 128, "bf16"), (9, 3, 64, "bf16"), (9, 3, 64, "f32"), (3, 1, 20, "bf16"), (2, 1, 256, "f32"), (40, 1, 32, "bf16")])
+def test_shares_of_the_sums(shares, window, heads, kv, dim, kind, monkeypatch):
+    monkeypatch.setattr(cache4(), "shares_of", lambda *a: shares)
+    check_step([3, 1, 2], [40, 0, 300], heads, kv, dim, 16, kind, window=window, weights=True)
+    check_step([150, 1, 40], [10, 70, 200], heads, kv, dim, 16, kind, window=window, weights=True)
 
 
 # -- which keys stay ----------------------------------------------------------------------------------------------
