@@ -33,6 +33,9 @@ def main(argv=None):
     parser.add_argument("--policy", choices=["serial", "chunked", "decode_first"], default="decode_first")
     parser.add_argument("--pages", type=int, default=128, help="cache pages; 0: as many as fit into the free GPU memory")
     parser.add_argument("--page-size", type=int, default=16)
+    parser.add_argument("--cache-bits", type=int, choices=[4], help="hold cached keys and values in 4 bits (else in the activations' type)")
+    parser.add_argument("--keep-keys", type=int, default=0, help="with --cache-bits 4: keys a request keeps, those with the most attention weight; 0: all")
+    parser.add_argument("--keep-recent", type=int, help="of --keep-keys, the last ones, which stay whatever their weight (a quarter unless given)")
     parser.add_argument("--token-budget", type=int, default=32)
     parser.add_argument("--prefill-chunk", type=int, default=8)
     parser.add_argument("--max-active", type=int, default=8)
@@ -54,7 +57,8 @@ def main(argv=None):
     execution = "graph" if args.execution == "graph" else "eager"
     common = dict(dtype=args.dtype, pages=args.pages, page_size=args.page_size, execution=execution,
                   policy=args.policy, token_budget=args.token_budget, prefill_chunk=args.prefill_chunk,
-                  max_active=args.max_active, overlap=args.overlap)
+                  max_active=args.max_active, overlap=args.overlap, cache_bits=args.cache_bits, keep_keys=args.keep_keys,
+                  keep_recent=args.keep_recent)
     if args.checkpoint:
         raw = read_config_json(args.checkpoint)
         engine = Engine.from_folder(args.checkpoint, **common)

@@ -26,6 +26,7 @@ class Appended:
     count: int
     slots: dict = field(default_factory=dict)   # group id -> [count] physical token slots
     state_slot: int = 0
+    dropped: int = 0                            # keys that were given up before: its first new token is key start - dropped
 
 
 class CacheManager:
@@ -52,7 +53,12 @@ class CacheManager:
             self.groups.append(group)
             for index, site in enumerate(sites):
                 self.group_of_site[site] = (gid, index)
+        keeps = {(getattr(need, "keep", 0), getattr(need, "slack", 0)) for need in by_need}
+        if len(keeps) > 1 or (keeps and max(keeps)[0] and any(need.window is not None for need in by_need)):
+            raise ValueError("sites that keep a bounded number of keys share the bound, and have no windows")
+        self.keep, self.slack = max(keeps) if keeps else (0, 0)
         self.lengths = {}
+        self.dropped = {}     # request -> tokens whose keys were given up (a request that has given up some)
         self.slots = StateSlots(max_requests)
         self.state_needs = dict(state_needs or {})
         self.state_storage = {}
@@ -86,6 +92,8 @@ class CacheManager:
             raise ValueError(f"duplicate request {target!r}")
         slot = self.slots.acquire(target)
         self.lengths[target] = self.lengths[source]
+        if source in self.dropped:
+            self.dropped[target] = self.dropped[source]
         for group in self.groups:
             group.fork(source, target)
         self._move_states(self.state_storage.values(), self.slots.slot_of(source), slot)
@@ -95,6 +103,7 @@ class CacheManager:
         """Give back everything the request holds.  The caller makes sure no
         device work that reads its pages is still running."""
         del self.lengths[request]
+        self.dropped.pop(request, None)
         for group in self.groups:
             group.release(request)
         self.slots.release(request)
@@ -105,6 +114,24 @@ class CacheManager:
     def length(self, request):
         return self.lengths[request]
 
+    def cached(self, request):
+        """Keys that the request holds (its length, less what it has given up)."""
+        return self.lengths[request] - self.dropped.get(request, 0)
+
+    def overfull(self, request):
+        """Whether the request holds more keys than its bound and the slack together."""
+        return self.keep > 0 and self.cached(request) > self.keep + self.slack
+
+    def give_up(self, request):
+        """All but `keep` of the request's keys go: per group (old block table, new block table), the pages of the old ones back in the pool.
+        The caller moves the kept keys, on the stream that every later user of those pages is ordered behind.  OutOfPages, with nothing
+        changed, where the kept keys find no pages."""
+        need = -(-self.keep // self.page_size)
+        if any(len(group.pool.free) < need for group in self.groups):
+            raise OutOfPages("no free KV pages for the keys that stay")
+        self.dropped[request] = self.lengths[request] - self.keep
+        return [group.exchange(request, self.keep) for group in self.groups]
+
     # -- appending ----------------------------------------------------------
     def pages_needed(self, items):
         """Per group: fresh pages minus pages a window gives back first."""
@@ -112,7 +139,7 @@ class CacheManager:
         for group in self.groups:
             need = 0
             for request, n in items:
-                length = self.lengths[request]
+                length = self.cached(request)
                 need += group.pages_needed(request, length, n) - group.trimmable(request, length)
             out.append(need)
         return out
@@ -146,9 +173,9 @@ class CacheManager:
         result, copied = [], {}
         for request, n in items:
             length = self.lengths[request]
-            done = Appended(request, length, n, state_slot=self.slots.slot_of(request))
+            done = Appended(request, length, n, state_slot=self.slots.slot_of(request), dropped=self.dropped.get(request, 0))
             for gid, group in enumerate(self.groups):
-                slots, copies = group.append(request, length, n)
+                slots, copies = group.append(request, length - done.dropped, n)
                 done.slots[gid] = slots
                 if copies:
                     copied.setdefault(gid, []).extend(copies)
@@ -183,7 +210,7 @@ class CacheManager:
         owner launches everything on ONE stream (ModelRunner refuses a step on another), which is that order.
         Per-request state is not restored: see ModelRunner.step."""
         for d in done:
-            keep = -(-self.lengths[d.request] // self.page_size)
+            keep = -(-self.cached(d.request) // self.page_size)
             for group in self.groups:
                 table = group.tables[d.request]
                 while len(table) > keep:
@@ -194,26 +221,28 @@ class CacheManager:
         """append_many, once windows have given back what they can, for the common step in which every request brings one
         token: the same pages in the same order, with the counting and the placing done in line."""
         P = self.page_size
-        lengths = self.lengths
+        lengths, dropped = self.lengths, self.dropped
+        held = {request: lengths[request] - dropped[request] for request, _ in items if request in dropped} if dropped else {}
+        held = {**lengths, **held} if held else lengths
         for group in self.groups:
             refs, tables, fresh = group.pool.refs, group.tables, 0
             for request, _ in items:
-                if lengths[request] % P == 0 or refs[tables[request][-1]] > 1:
+                if held[request] % P == 0 or refs[tables[request][-1]] > 1:
                     fresh += 1
             if fresh > len(group.pool.free):
                 raise OutOfPages("not enough free KV pages for this step")
         result, copied = [], {}
         for request, _ in items:
-            length = lengths[request]
-            done = Appended(request, length, 1, state_slot=self.slots.slot_of(request))
+            length, cached = lengths[request], held[request]
+            done = Appended(request, length, 1, state_slot=self.slots.slot_of(request), dropped=length - cached)
             for gid, group in enumerate(self.groups):
                 table = group.tables[request]
-                if length % P == 0:
+                if cached % P == 0:
                     table.append(group.pool.allocate())
                     group._touch(request)
                 elif group.pool.refs[table[-1]] > 1:      # the shared, partly filled last page: copy on write
-                    copied.setdefault(gid, []).extend(group.append(request, length, 1)[1])
-                done.slots[gid] = [table[-1] * P + length % P]
+                    copied.setdefault(gid, []).extend(group.append(request, cached, 1)[1])
+                done.slots[gid] = [table[-1] * P + cached % P]
             if commit:
                 lengths[request] = length + 1
             result.append(done)
@@ -244,7 +273,7 @@ class CacheManager:
             group.check()
             assert set(group.tables) == set(self.lengths), "a group knows other requests than the manager"
             for request, table in group.tables.items():
-                assert len(table) == -(-self.lengths[request] // group.page_size), "table length differs from token count"
+                assert len(table) == -(-self.cached(request) // group.page_size), "table length differs from token count"
         self.slots.check()
         assert set(self.slots.owner) == set(self.lengths)
 
@@ -252,8 +281,8 @@ class CacheManager:
         return [len(g.pool.free) for g in self.groups]
 
     def capacity(self):
-        """Pages of each group's pool."""
-        return [g.pool.n_pages for g in self.groups]
+        """Pages of each group's pool that requests can be promised: all but what the kept keys of one request move to (give_up)."""
+        return [g.pool.n_pages - -(-self.keep // self.page_size) for g in self.groups]
 
     def most_pages_held(self, tokens, portion):
         """Per group, the most pages one request holds at any time while it grows to `tokens` cached tokens in
@@ -267,6 +296,8 @@ class CacheManager:
             if group.need.window is not None:
                 kept = -(-getattr(group.need, "keep_first", 0) // P)
                 pages = min(pages, kept + (group.need.window + max(1, portion) - 1) // P + 2)
+            if self.keep:
+                pages = min(pages, -(-(self.keep + self.slack + max(1, portion)) // P))
             out.append(pages)
         return out
 
@@ -285,7 +316,8 @@ def pages_that_fit(site_needs, page_size, itemsize, free_bytes, fraction=0.8, mo
     """How many pages a pool may have so that the caches of all sites take `fraction` of `free_bytes`:
     a page index costs, in every site that keeps pages, page_size times the elements its need takes a token.
     `most` caps the answer (more pages than the requests can ever address are of no use)."""
-    per_page = sum(need.elements_per_token() * page_size * itemsize for need in site_needs.values() if need is not None)
+    per_page = sum((need.bytes_per_token(itemsize) if hasattr(need, "bytes_per_token") else need.elements_per_token() * itemsize) * page_size
+                   for need in site_needs.values() if need is not None)
     if per_page == 0:
         return 1
     pages = int(free_bytes * fraction) // per_page

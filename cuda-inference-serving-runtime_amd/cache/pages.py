@@ -76,6 +76,29 @@ class KeptWindowNeed(KVNeed):
 
 
 @dataclass(frozen=True)
+class FourBitNeed(KVNeed):
+    """Keys and values held in 4 bits (kernels/cache4.py): one run of bytes a page and head.  With `keep` a request holds a bounded
+    number of keys: after a step that leaves it more than `keep` + `slack`, the owner gives up all but `keep` of them."""
+    keep: int = 0
+    slack: int = 0
+    storage_dtype = "uint8"
+
+    def bytes_per_token(self, itemsize):
+        pad = -(-self.head_dim // 32) * 32
+        return self.kv_heads * (pad + pad // 16)
+
+    def storage_shape(self, sites, pages, page_size):
+        return (sites, pages, self.kv_heads, self.bytes_per_token(1) // self.kv_heads * page_size)
+
+    def slabs(self, sites):
+        return sites
+
+    def views(self, storage, index):
+        """The pages [pages, kv_heads, bytes] of site `index`."""
+        return (storage[index],)
+
+
+@dataclass(frozen=True)
 class StateNeed:
     """A fixed-size state per request."""
     shape: tuple
@@ -246,6 +269,14 @@ class CacheGroup:
         else:
             slots = [table[(length + i) // P] * P + (length + i) % P for i in range(n_new)]
         return slots, copies
+
+    def exchange(self, request, tokens):
+        """Fresh pages for the first `tokens` tokens in the place of all that the request holds: (old table, new table); the old pages go back."""
+        old, new = self.tables[request], self.pool.allocate_many(-(-tokens // self.page_size))
+        self.tables[request] = list(new)
+        self.pool.drop_all(old)
+        self._touch(request)
+        return old, new
 
     def create(self, request):
         self.tables[request] = []

@@ -48,6 +48,8 @@ class Batch:
     launch_values: dict   # StepArray -> its launch value for this step
     rows: int = 0         # rows that the step is padded to (0: not padded)
     made: dict = field(default_factory=dict)      # what one array's filling may leave for another's of this step
+    cached: list = None   # keys that each segment's request holds before its first new token (fewer than `starts` where some were given up)
+    slots: list = None    # each segment's state slot
 
 
 class StepContext:

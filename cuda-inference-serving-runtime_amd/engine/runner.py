@@ -18,8 +18,8 @@ from typing import List, Sequence
 import numpy as np
 import torch
 
-from ..cache import CacheManager
-from ..kernels import ops
+from ..cache import CacheManager, OutOfPages
+from ..kernels import cache4, ops
 from .context import Batch, GroupView, StepContext, Workspace
 
 
@@ -74,13 +74,19 @@ class ModelRunner:
         self.max_requests = max_requests
         dtype = model.dtype
 
+        needs = model.cache_needs()
+        held = {getattr(need, "storage_dtype", None) for need in needs.values()}
+        if len(held) > 1:
+            raise ValueError("layers that hold their caches in different types")
+        stored = torch.uint8 if held == {"uint8"} else dtype
+
         def allocate_pages(shape):
-            return torch.zeros(shape, dtype=dtype, device=self.device)
+            return torch.zeros(shape, dtype=stored, device=self.device)
 
         def allocate_state(slots, shape, dt):
             return torch.zeros((slots, *shape), dtype=_TORCH_OF[dt], device=self.device)
 
-        self.cache = CacheManager(model.cache_needs(), n_pages, page_size, max_requests,
+        self.cache = CacheManager(needs, n_pages, page_size, max_requests,
                                   state_needs=model.state_needs(), allocate_pages=allocate_pages,
                                   allocate_state=allocate_state, copy_pages=self._copy_pages,
                                   move_states=ops.move_states)
@@ -136,6 +142,8 @@ class ModelRunner:
             raise ValueError("a step needs at least one entry")
         seen = set()
         vocab, limit, lengths = self.model.vocab_size, self.max_context, self.cache.lengths
+        kept = getattr(self.model, "kept_keys", None)
+        most = kept[0] + self.cache.slack + kept[2] if kept else 0
         for e in entries:
             if e.request in seen:
                 raise ValueError(f"request {e.request!r} appears twice in one step")
@@ -150,6 +158,9 @@ class ModelRunner:
                 raise ValueError(f"request {e.request!r} brings no tokens")
             if lengths[e.request] + n > limit:
                 raise ValueError(f"request {e.request!r} exceeds the context limit of {limit}")
+            if most and self.cache.cached(e.request) + n > most:
+                raise ValueError(f"request {e.request!r} brings {n} tokens beside {self.cache.cached(e.request)} cached keys: at most {most} in all, "
+                                 f"of which it keeps {self.model.kept_keys[0]}")
             if e.pending:
                 if n != 1 or e.request not in self._has_picked:
                     raise ValueError(f"request {e.request!r} has no one token picked on the device")
@@ -195,11 +206,35 @@ class ModelRunner:
                 self._failed.update(e.request for e in entries)
             raise
         self.cache.commit(done)
+        if getattr(self.model, "kept_keys", None):
+            for d in done:
+                if self.cache.overfull(d.request):
+                    self._give_up(d.request)
         self.steps += 1
         self.counters["steps"] += 1
         if logits is None:
             return torch.empty((0, self.model.vocab_size), dtype=torch.float32, device=self.device)
         return logits
+
+    def _give_up(self, request):
+        """The request keeps the keys that its mixers' sums of attention weight speak for, at every site and head its own.  Where their new pages
+        find no room it keeps all for now (the next step tries again; a step that it would bring too many keys to is refused)."""
+        cache, (keep, recent, _) = self.cache, self.model.kept_keys
+        held, slot = cache.cached(request), cache.slots.slot_of(request)
+        try:
+            tables = cache.give_up(request)
+        except OutOfPages:
+            return
+        for group, (old, new) in zip(cache.groups, tables):
+            n, m = len(old), len(new)
+            host = self._stage(3 + n + m)
+            host[:3 + n + m] = torch.tensor([held, slot, slot, *old, *new], dtype=torch.int32)
+            dev = self._upload(host, 3 + n + m)
+            need = group.need
+            kept = self.workspace.get("cache4.kept", (len(group.sites), 1, need.kv_heads, keep), torch.int32)
+            cache4.evict(group.storage, [cache.state_storage[site] for site in group.sites], dev[3:3 + n][None], dev[3 + n:3 + n + m][None], dev[:1], dev[1:2], dev[2:3],
+                         need.kv_heads, need.head_dim, self.page_size, keep, recent, kept)
+        self.counters["evictions_of_keys"] = self.counters.get("evictions_of_keys", 0) + 1
 
     def _forward(self, ctx, take):
         if take:   # rows whose token is still only on the device get it from there
@@ -260,7 +295,8 @@ class ModelRunner:
     def _launch_values(self, done):
         """What the parts' launches depend on beside rows, segments and contexts: the launch value of every carried
         step array that has one (context.StepArray), for this batch."""
-        batch = Batch([d.count for d in done], [d.start for d in done], None, all(d.count == 1 for d in done), {}, _bucket(sum(d.count for d in done)))
+        batch = Batch([d.count for d in done], [d.start for d in done], None, all(d.count == 1 for d in done), {}, _bucket(sum(d.count for d in done)),
+                      cached=[d.start - d.dropped for d in done])
         for array in self.carried:
             batch.launch_values[array] = array.launch_value(batch)
         return batch.launch_values
@@ -276,7 +312,7 @@ class ModelRunner:
         n_want = sum(len(e.want) for e in entries)
         T, S, R = pad if pad is not None else (n_rows, n_seg, n_want)
         # the longest context of the step (a captured program brings the bound of its bucket) sizes the block tables
-        longest = max(s + c for s, c in zip(starts, counts))
+        longest = max(s + c for s, c in zip(starts, counts)) if not self.cache.dropped else max(d.start - d.dropped + d.count for d in done)
         W, G, F = self._width(longest if context is None else context), len(self.cache.groups), self._FIXED
         carried = tuple(self.carried)
         layout = (T, S, R, W, carried)
@@ -338,7 +374,7 @@ class ModelRunner:
                 slots[n_rows:] = -1
                 tables[n_seg:] = -1
         # what the parts asked for: first every launch value, then the arrays (one may read another's value)
-        batch = Batch(counts, starts, first_row, decode_only, {}, T)
+        batch = Batch(counts, starts, first_row, decode_only, {}, T, cached=[d.start - d.dropped for d in done], slots=slot_of)
         for array in carried:
             own = array.launch_value(batch)
             batch.launch_values[array] = own if launch_values is None or own is None else launch_values.get(array, 0)
@@ -400,7 +436,7 @@ class ModelRunner:
         rows = sum(d.count for d in done)
         wanted = sum(len(e.want) for e in entries)
         decode_only = all(d.count == 1 for d in done)
-        context = 1 << (max(d.start + d.count for d in done) - 1).bit_length()
+        context = 1 << (max(d.start - d.dropped + d.count for d in done) - 1).bit_length()
         values = tuple((array, _bucket(value)) for array, value in self._launch_values(done).items() if value)
         return (_bucket(rows), _bucket(len(entries)), _bucket(wanted), decode_only, max(context, 256),
                 any(e.pending for e in entries), values)

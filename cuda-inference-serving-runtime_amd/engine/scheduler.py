@@ -124,6 +124,9 @@ class Engine:
                 raise ValueError(f"{name} must be positive, not {value}")
         if policy not in POLICIES:
             raise ValueError(f"policy {policy!r} is none of {POLICIES}")
+        kept = getattr(runner.model, "kept_keys", None)
+        if kept and min(prefill_chunk, token_budget) > kept[2]:
+            raise ValueError(f"prompts in portions of {min(prefill_chunk, token_budget)}: the model's cache was made for at most {kept[2]} (hold_cache)")
         self.runner = runner
         self.max_active = 1 if policy == "serial" else min(max_active, runner.max_requests)
         self.token_budget, self.prefill_chunk, self.policy = token_budget, prefill_chunk, policy
@@ -323,23 +326,31 @@ class Engine:
 
     # -- conveniences ---------------------------------------------------------------
     @classmethod
-    def from_folder(cls, folder, dtype="bfloat16", pages=128, page_size=16, execution="graph", device="cuda:0", **limits):
+    def from_folder(cls, folder, dtype="bfloat16", pages=128, page_size=16, execution="graph", device="cuda:0", cache_bits=None,
+                    keep_keys=0, keep_recent=None, **limits):
         """An engine for the model in `folder` (config.json + safetensors).  Steps run as captured programs unless
         execution="eager" (kernels launched one by one).  pages None (or 0): as many as fit
         into four fifths of the GPU memory that is free once the weights are loaded, at most what the
-        requests can address."""
+        requests can address.  `cache_bits` 4: the cache holds keys and values in 4 bits; `keep_keys`: and about that many keys a request, those
+        with the most attention weight and the last `keep_recent` (a quarter of them unless given)."""
         import torch
         from ..cache import pages_that_fit
         from .loading import load_model
         from .runner import ModelRunner
         model = load_model(folder, dtype=dtype, device=device)
+        if cache_bits is not None:
+            # (what a step brings a request at most: Engine's own limits, see __init__)
+            portion = max(1, min(limits.get("prefill_chunk", 8), limits.get("token_budget", 32)))
+            model.hold_cache(cache_bits, keep_keys, keep_recent, portion=portion)
+        elif keep_keys:
+            raise ValueError("a bounded number of keys is kept by the cache of 4 bits (cache_bits=4)")
         max_requests = max(8, limits.get("max_active", 8))
         if not pages:
             free, _ = torch.cuda.mem_get_info(torch.device(device))
             addressable = max_requests * -(-model.max_positions // page_size)
             # (the attention kernels address a site's keys with 32-bit byte offsets: fewer than 2^31 elements;
             # a model whose mixers keep no keys has nothing to size)
-            widths = [need.kv_heads * need.head_dim for need in model.cache_needs().values() if need is not None]
+            widths = [need.kv_heads * need.head_dim for need in model.cache_needs().values() if need is not None and not hasattr(need, "storage_dtype")]
             if widths:
                 by_offsets = (2 ** 31 - 1) // (max(widths) * page_size)
                 if by_offsets < addressable:

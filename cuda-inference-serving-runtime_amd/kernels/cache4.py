@@ -433,3 +433,119 @@ def evict(storage, weights, tables, new_tables, lengths, slots, new_slots, kv_he
                 _t(kept, "kept", torch.int32, (sites, requests, kv_heads, keep), index), sites, n, requests, kv_heads, dim, page_size, tables.shape[1],
                 new_tables.shape[1], keep, recent, capacity, n_slots)
     return kept
+
+
+# -- a step of the engine -----------------------------------------------------------------------------------------------
+
+@dataclass(frozen=True)
+class StepForm:
+    """Step array without words whose launch value says how a step's rows are taken: 2 to the power of twice the form, and once more where
+    keys are in several pieces (powers of two: captured programs round launch values up to them)."""
+    pieces: "StepPieces"
+
+    def words(self, rows, segments):
+        return 0
+
+    def launch_value(self, batch):
+        _, merges, form = self.pieces.made(batch)
+        return 1 << (2 * form + (1 if len(merges) else 0))
+
+    def fill(self, out, batch, value):
+        pass
+
+
+@dataclass(frozen=True)
+class StepPieces:
+    """Step array: the tasks of a step (see fill_pieces), then, from the end backwards, its merges.  Its launch value is the number of tasks."""
+    heads: int
+    kv_heads: int
+    dim: int
+    window: int
+    half: bool                 # rows in bfloat16
+
+    def launch(self, rows, segments, decode_only):
+        """(form, rows of a task, pieces) for a step."""
+        form, per_task = launch_of(rows, segments, decode_only, self.heads, self.kv_heads, self.dim, torch.bfloat16 if self.half else torch.float32)
+        return form, per_task, pieces_for(self.kv_heads, self.heads // self.kv_heads, per_task, form, decode_only)
+
+    def most(self, rows, segments):
+        """(tasks, merges) at most: of a step of single tokens, or of prompts by the smallest tiles."""
+        group = self.heads // self.kv_heads
+        tasks, tiles = zip(most_tasks(rows, segments, 1, pieces_for(self.kv_heads, group, 1, 0, True)) if rows == segments else (0, 0),
+                           most_tasks(rows, segments, max(1, 16 // group), 2 * COMPUTE_UNITS))
+        return max(tasks), max(tiles)
+
+    def made(self, batch):
+        """(tasks, merges, form) of the batch."""
+        got = batch.made.get(self)
+        if got is None:
+            rows, segments = sum(batch.counts), len(batch.counts)
+            form, per_task, pieces = self.launch(batch.rows or rows, segments, batch.decode_only)
+            tasks, merges = (np.empty((n, k), dtype=np.int32) for n, k in zip(most_tasks(rows, segments, per_task, pieces), (8, 4)))
+            n, m = fill_pieces(tasks, merges, batch.counts, batch.cached, per_task, pieces, self.window)
+            got = batch.made[self] = (tasks[:n], merges[:m], form)
+        return got
+
+    def words(self, rows, segments):
+        tasks, merges = self.most(rows, segments)
+        return 8 * tasks + 4 * merges
+
+    def launch_value(self, batch):
+        return len(self.made(batch)[0])
+
+    def fill(self, out, batch, value):
+        tasks, merges, _ = self.made(batch)
+        out[:] = -1
+        out[:8 * len(tasks)] = tasks.reshape(-1)
+        if len(merges):
+            out[len(out) - 4 * len(merges):] = merges.reshape(-1)
+
+
+@dataclass(frozen=True)
+class StepSegments:
+    """Step array: int32 [S, 4] of first row, rows, keys before the first row and state slot of every segment; no rows pad it."""
+
+    def words(self, rows, segments):
+        return 4 * segments
+
+    def launch_value(self, batch):
+        return None
+
+    def fill(self, out, batch, value):
+        out[:] = 0
+        n = len(batch.counts)
+        out[:4 * n] = np.stack([batch.first_row, batch.counts, batch.cached, batch.slots], 1).reshape(-1)
+
+
+def step_arrays(heads, kv_heads, dim, window, operand, sums):
+    """What `attend` wants of every step, for a layer whose output projection's weights are `operand` (their type is the rows')."""
+    if operand is None:
+        return []
+    pieces = StepPieces(heads, kv_heads, dim, _window(window), operand.dtype is torch.bfloat16)
+    return [pieces, StepForm(pieces)] + ([StepSegments()] if sums else [])
+
+
+def attend(ctx, q, pages, view, out, heads, kv_heads, dim, scale, window=None, sums=None):
+    """`attention` of a step's rows, and with `sums` (float [slots, kv_heads, capacity]) `add_weights`.  `ctx` is the step's context, `view`
+    the cache group as the step sees it."""
+    array = StepPieces(heads, kv_heads, dim, _window(window), q.dtype is torch.bfloat16)
+    words, n_tasks = ctx.step_array(array)
+    _, flags = ctx.step_array(StepForm(array))
+    form, split = divmod(flags.bit_length() - 1, 2)
+    most, merges = array.most(ctx.n_rows, ctx.n_segments)
+    per_task = 1 if ctx.decode_only else max(1, tile_of(form) // (heads // kv_heads))
+    rows, S = ctx.n_rows, ctx.n_segments
+    shares, span, segments = 0, ctx.span_hint, None
+    if sums is not None:
+        segments = ctx.step_array(StepSegments())[0].view(S, 4)
+        span = min(span, sums.shape[2])
+        shares = shares_of(rows, S, span, heads // kv_heads, kv_heads)
+    pieces = n_tasks if split else 0
+    floats = max(pieces * per_task * heads * (dim + 2), shares * S * kv_heads * span if shares > 1 else 0)
+    plan = Plan(rows, S, span, heads, kv_heads, dim, form, per_task, words[:8 * min(n_tasks, most)].view(-1, 8), words[len(words) - 4 * merges:].view(-1, 4) if split else None,
+                pieces, segments, 0 if sums is None else sums.shape[0], shares, ctx.buffer("cache4.room", (floats,), torch.float32) if floats else None)
+    stats = None if sums is None else ctx.buffer("cache4.stats", (rows, heads), torch.float32)
+    attention(q, pages, view.tables, plan, out, heads, kv_heads, dim, view.page_size, scale, window, stats)
+    if sums is not None:
+        add_weights(q, stats, pages, view.tables, plan, sums, heads, kv_heads, dim, view.page_size, scale, window)
+    return out

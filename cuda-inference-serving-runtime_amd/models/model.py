@@ -78,6 +78,31 @@ class Model:
             part.bind(tensors, dtype)
             part.prepare(device, dtype)
 
+    def hold_cache(self, bits=4, keep=0, recent=None, slack=64, portion=2048):
+        """Before a runner is made: the cache holds keys and values in 4 bits (kernels/cache4.py).  With `keep` a request holds that many
+        keys and at most `slack` more between steps: beyond that, every layer and head gives up the keys with the least attention weight so far, but
+        none of the last `recent` (a quarter of `keep` unless given); a step brings a request at most `portion` tokens then."""
+        if bits != 4:
+            raise ValueError(f"a cache of {bits} bits: 4, or the activations' type")
+        recent = keep // 4 if recent is None else recent
+        if keep < 0 or not 0 <= recent <= keep or (keep and (slack <= 0 or portion <= 0)):
+            raise ValueError(f"keeping {keep} keys, {recent} of them the last, with {slack} more between steps and portions of {portion}")
+        mixers = [getattr(layer, "mixer", None) for layer in self.layers]
+        if any(not hasattr(mixer, "hold_in_4_bits") for mixer in mixers):
+            raise ValueError("a layer whose keys and values cannot be held in 4 bits")
+        done = []
+        try:
+            for mixer in mixers:
+                mixer.hold_in_4_bits(keep, slack, portion)
+                done.append(mixer)
+        except ValueError:
+            for mixer in done:
+                mixer.four_bits = None
+            raise
+        self.kept_keys = (keep, recent, portion) if keep else None
+
+    kept_keys = None      # (keys that a request keeps, of them the last, tokens that a step may bring), or None: all
+
     # -- what the cache manager must provide ------------------------------------
     def site_of(self, index):
         entry = self.schedule[index]

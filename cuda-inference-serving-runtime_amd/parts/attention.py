@@ -17,8 +17,8 @@ import math
 
 import torch
 
-from ..cache.pages import ChunkNeed, KeptWindowNeed, KVNeed
-from ..kernels import attention as kernel, ops
+from ..cache.pages import ChunkNeed, FourBitNeed, KeptWindowNeed, KVNeed, StateNeed
+from ..kernels import attention as kernel, cache4, ops
 from .base import Mixer, TensorSpec, matrix_operand, register_part, runs_own
 
 
@@ -35,15 +35,31 @@ class PagedAttention(Mixer):
         self.bias, self.out_bias = bool(bias), bool(out_bias)
         self.w_in = self.w_out = self.b_in = self.b_out = self.merges = None
         self.tuning = tuning if tuning is not None else kernel.DEFAULT_TUNING   # what the kernel's launch rules may be told
+        self.four_bits = None      # (keys kept, slack, a step's tokens): the cache holds keys and values in 4 bits
+
+    def hold_in_4_bits(self, keep, slack, portion):
+        if not cache4.supported(self.head_dim, 8):
+            raise ValueError(f"{self.name}: heads of {self.head_dim} are not held in 4 bits")
+        if keep and (self.window is not None or not self.own_kv):
+            raise ValueError(f"{self.name}: a bounded number of keys is kept by layers without a window that have keys of their own")
+        self.four_bits = (keep, slack, portion)
 
     def kernel_units(self, dtype):
-        return kernel.kernel_units(self.head_dim, dtype)
+        return [cache4.UNIT] if self.four_bits else kernel.kernel_units(self.head_dim, dtype)
 
     def step_arrays(self):
+        if self.four_bits:
+            return cache4.step_arrays(self.heads, self.kv_heads, self.head_dim, self.window, self.w_out, self.four_bits[0] > 0)
         return kernel.step_arrays(self.tuning, self.w_out, self.heads, self.kv_heads, self.head_dim, self.window, 0, self.merges)
 
     def cache_need(self):
+        if self.own_kv and self.four_bits:
+            return FourBitNeed(self.kv_heads, self.head_dim, self.window, *self.four_bits[:2])
         return KVNeed(self.kv_heads, self.head_dim, self.window) if self.own_kv else None
+
+    def state_need(self):
+        # every key's attention weight so far, by key head
+        return StateNeed((self.kv_heads, sum(self.four_bits))) if self.four_bits and self.four_bits[0] else None
 
     def cache_read(self):
         return None if self.own_kv else KVNeed(self.kv_heads, self.head_dim, self.window)
@@ -84,7 +100,7 @@ class PagedAttention(Mixer):
     def _fused_projection_ok(self, a, normed, scratch, weight=None):
         cos, sin = self.position.tables()
         # (the fused kernels turn split-half pairs only; another pairing takes the general rotary kernel)
-        if self._interleaved or self.bias:
+        if self._interleaved or self.bias or self.four_bits:
             return False
         return ops.qkv_rope_fused_ok(a, self.w_in, self.head_dim, cos, normed, scratch, sin, weight) or (not normed and ops.qkv_rope_f32_ok(a, self.w_in, self.head_dim, cos))
 
@@ -94,11 +110,16 @@ class PagedAttention(Mixer):
     def takes_scaled(self, rows, ctx):
         """Whether this step's projection of the rows `rows` can finish their norm (ops.ScaledRows)."""
         cos, sin = self.position.tables()
-        return runs_own(self, PagedAttention) and not (self._interleaved or self.bias) and ops._ring_open(ctx.scratch) and ops.ring_rope_ok(rows, self.w_in, self.head_dim, cos, sin)
+        return runs_own(self, PagedAttention) and not (self._interleaved or self.bias or self.four_bits) and ops._ring_open(ctx.scratch) and ops.ring_rope_ok(rows, self.w_in, self.head_dim, cos, sin)
 
     def forward(self, h, residual, ctx, site, norm=None):
         T = residual.shape[0]
         D, nh, nkv = self.head_dim, self.heads, self.kv_heads
+        if self.four_bits:
+            residual = ctx.add_product(self._attend_4_bits(h, ctx, site), self.w_out, residual, last=self if self.b_out is None else None, of=PagedAttention)
+            if self.b_out is not None:
+                ops.bias_add(residual, self.b_out)
+            return residual
         gid, kcache, vcache = ctx.cache.pages_of_site(site)
         view = ctx.kv[gid]
         cos, sin = self.position.tables()
@@ -132,6 +153,26 @@ class PagedAttention(Mixer):
         if self.b_out is not None:
             ops.bias_add(residual, self.b_out)   # (sums commute: slices of the product that a later norm adds may still be out; its norm is not taken yet)
         return residual
+
+
+    def _attend_4_bits(self, h, ctx, site):
+        """The heads' results [T, heads * head_dim] over a cache in 4 bits."""
+        T, D, nh, nkv = h.shape[0], self.head_dim, self.heads, self.kv_heads
+        gid, pages = ctx.cache.pages_of_site(site)
+        view = ctx.kv[gid]
+        cos, sin = self.position.tables()
+        rows = ctx.buffer("attn.qkv", (T, self.w_in.shape[0]), ctx.dtype)
+        ops.gemm(h, self.w_in, rows, scratch=ctx.scratch)
+        if self.b_in is not None:
+            ops.bias_add(rows, self.b_in)
+        if self.own_kv:
+            q = ctx.buffer("attn.q", (T, nh * D), ctx.dtype)
+            cache4.rope_write(rows, ctx.positions, view.slots, cos, sin, pages, q, nh, nkv, D, view.page_size, interleaved=self._interleaved)
+        else:
+            q = rows
+            ops.rope_scatter(q, ctx.positions, None, cos, sin, None, None, nh, nkv, D, view.page_size, interleaved=self._interleaved)
+        sums = ctx.cache.state_storage[site] if self.four_bits[0] else None
+        return cache4.attend(ctx, q, pages, view, ctx.buffer("attn.out", (T, nh * D), ctx.dtype), nh, nkv, D, self.scale, self.window, sums)
 
 
 class NormedGatedAttention(Mixer):

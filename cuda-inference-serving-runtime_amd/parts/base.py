@@ -76,6 +76,11 @@ class Mixer(Part):
     def state_need(self):
         return None
 
+    def hold_in_4_bits(self, keep, slack, portion):
+        """Have the cache hold keys and values in 4 bits; `keep` > 0: a bounded number of keys a request, with room for `slack` and a step's
+        `portion` of tokens beyond it."""
+        raise ValueError(f"{type(self).__name__} holds its keys and values in the activations' type only")
+
     def fuses_norm(self, norm, residual, ctx):
         return False
 
