@@ -23,15 +23,76 @@ __device__ __forceinline__ uint32_t cache4_codes(const float (&x)[8], int& s) {
     most = fmaxf(most, __shfl_xor(most, 1, WAVE));
     most = fmaxf(most, __shfl_xor(most, 2, WAVE));
     s = min(max((int)((__float_as_uint(most) + 0x1fffffu) >> 23) - 129, -125), 125);
-    const float inv = __uint_as_float((uint32_t)(127 - s) << 23);
-    uint32_t word = 0;
+    // the conversion rounds to the nearest, ties to the even code, and stops at 6; it takes a NaN for 6 and keeps the sign of a zero
+    float sum = 0.f, y[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float y = fabsf(x[i]) * inv;
-        const uint32_t code = (y > 0.25f) + (y >= 0.75f) + (y > 1.25f) + (y >= 1.75f) + (y > 2.5f) + (y >= 3.5f) + (y > 5.f);
-        word |= (code | (x[i] < 0.f ? 8u : 0u)) << (4 * i);
+    for (int i = 0; i < 8; ++i) { y[i] = x[i] + 0.f; sum += y[i]; }
+    if (sum != sum)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = x[i] != x[i] ? 0.f : y[i];
+    const float scale = __uint_as_float((uint32_t)(127 + s) << 23);
+    uint32_t word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, y[0], y[1], scale, 0);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[2], y[3], scale, 1);
+    word = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[4], y[5], scale, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(word, y[6], y[7], scale, 3);
+}
+
+// Eight coordinates from c0 on of a token's key or value, with their scale, to their places.  (The four threads of a block call it together.)
+__device__ __forceinline__ void cache4_put(const Write4Args& p, int slot, int head, bool value, int c0, const float (&y)[8]) {
+    int s;
+    const uint32_t word = cache4_codes(y, s);
+    if (slot < 0 || slot >> p.shift >= p.n_pages) return;
+    const int t = slot & ((1 << p.shift) - 1);
+    uint8_t* page = p.pages + ((size_t)(slot >> p.shift) * p.kv_heads + head) * cache4_record(p.dp, 1 << p.shift);
+    if (c0 % 32 == 0) page[cache4_scale_at(p.dp, p.shift, t, c0 / 32, value)] = (uint8_t)(s + CACHE4_BIAS);
+    if (!value) {
+        *(uint32_t*)(page + cache4_key_at(p.dp, t, c0)) = word;
+        return;
     }
-    return word;
+    const int w = cache4_cut(p.dp) / 16;
+    if (w == 8) {
+        *(uint32_t*)(page + cache4_value_at(p.dp, p.shift, t, c0)) = word;
+    } else if (w == 4) {
+        for (int i = 0; i < 2; ++i) *(uint16_t*)(page + cache4_value_at(p.dp, p.shift, t, c0 + 4 * i)) = (uint16_t)(word >> (16 * i));
+    } else {
+        for (int i = 0; i < 4; ++i) page[cache4_value_at(p.dp, p.shift, t, c0 + 2 * i)] = (uint8_t)(word >> (8 * i));
+    }
+}
+
+// Whole heads turn, in halves of whole blocks: a thread has eight coordinates of either half, the pairs that turn together.
+template <typename T>
+__global__ void __launch_bounds__(256)
+write4_halves_kernel(Write4Args p) {
+#pragma clang fp contract(off)
+    const uint32_t per_head = p.dim / 16, all = p.heads + 2 * p.kv_heads, at = blockIdx.x * 256 + threadIdx.x, vector = at / per_head, row = vector / all;
+    if (row >= (uint32_t)p.rows) return;                           // (whole blocks of 32 coordinates: their four threads leave together)
+    const int c0 = 8 * (int)(at - vector * per_head), h = (int)(vector - row * all), half = p.dim / 2;
+    const T* x = (const T*)p.qkv + (size_t)vector * p.dim;
+    float a[8], b[8];
+    load_run<4>(x + c0, *(float (*)[4])a); load_run<4>(x + c0 + 4, *(float (*)[4])(a + 4));
+    load_run<4>(x + half + c0, *(float (*)[4])b); load_run<4>(x + half + c0 + 4, *(float (*)[4])(b + 4));
+    const bool value = h >= p.heads + p.kv_heads;
+    if (!value) {
+        const size_t pos = (size_t)min(max(p.positions[row], 0), p.max_pos - 1) * half + c0;
+        float cs[8], sn[8];
+        load_run<4>(p.cos + pos, *(float (*)[4])cs); load_run<4>(p.cos + pos + 4, *(float (*)[4])(cs + 4));
+        load_run<4>(p.sin + pos, *(float (*)[4])sn); load_run<4>(p.sin + pos + 4, *(float (*)[4])(sn + 4));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float ac = a[i] * cs[i], bs = b[i] * sn[i], bc = b[i] * cs[i], as = a[i] * sn[i];
+            a[i] = ac - bs;
+            b[i] = bc + as;
+        }
+        if (h < p.heads) {
+            T* q = (T*)p.q + ((size_t)row * p.heads + h) * p.dim;
+            store_run<4>(q + c0, *(float (*)[4])a); store_run<4>(q + c0 + 4, *(float (*)[4])(a + 4));
+            store_run<4>(q + half + c0, *(float (*)[4])b); store_run<4>(q + half + c0 + 4, *(float (*)[4])(b + 4));
+            return;
+        }
+    }
+    const int slot = p.slots[row], head = h - p.heads - (value ? p.kv_heads : 0);
+    cache4_put(p, slot, head, value, c0, a);
+    cache4_put(p, slot, head, value, half + c0, b);
 }
 
 template <typename T, bool WORDS>
@@ -99,27 +160,8 @@ write4_kernel(Write4Args p) {
         }
         return;
     }
-    const int slot = p.slots[row];
     const bool value = h >= p.heads + p.kv_heads;
-    const int head = h - p.heads - (value ? p.kv_heads : 0);
-    int s;
-    const uint32_t word = cache4_codes(y, s);
-    if (slot < 0 || slot >> p.shift >= p.n_pages) return;
-    const int t = slot & ((1 << p.shift) - 1);
-    uint8_t* page = p.pages + ((size_t)(slot >> p.shift) * p.kv_heads + head) * cache4_record(p.dp, 1 << p.shift);
-    if ((u & 3) == 0) page[cache4_scale_at(p.dp, p.shift, t, u / 4, value)] = (uint8_t)(s + CACHE4_BIAS);
-    if (!value) {
-        *(uint32_t*)(page + cache4_key_at(p.dp, t, c0)) = word;
-        return;
-    }
-    const int w = cache4_cut(p.dp) / 16;
-    if (w == 8) {
-        *(uint32_t*)(page + cache4_value_at(p.dp, p.shift, t, c0)) = word;
-    } else if (w == 4) {
-        for (int i = 0; i < 2; ++i) *(uint16_t*)(page + cache4_value_at(p.dp, p.shift, t, c0 + 4 * i)) = (uint16_t)(word >> (16 * i));
-    } else {
-        for (int i = 0; i < 4; ++i) page[cache4_value_at(p.dp, p.shift, t, c0 + 2 * i)] = (uint8_t)(word >> (8 * i));
-    }
+    cache4_put(p, p.slots[row], h - p.heads - (value ? p.kv_heads : 0), value, c0, y);
 }
 
 // What is held for the token slots `slots`, as bf16 (every held number is one).  A thread has 8 coordinates; a slot that is none gives zeros.
@@ -136,26 +178,22 @@ __device__ __forceinline__ uint4 cache4_eight(uint32_t word, int s) {
 
 struct Read4Args {
     const uint8_t* pages; const int* slots; bf16_t* keys; bf16_t* values;
-    long long vectors;                       // sites * rows * heads * 2
+    uint32_t pieces;                         // of a site: rows * heads * (keys, values) * eights of coordinates
     int rows, kv_heads, dim, dp, shift, n_pages;
 };
 
 __global__ void __launch_bounds__(256)
 read4_kernel(Read4Args p) {
-    const int per_head = (p.dim + 7) / 8;
-    const long long at = (long long)blockIdx.x * 256 + threadIdx.x, vector = at / per_head;
-    if (vector >= p.vectors) return;
-    const int c0 = 8 * (int)(at - vector * per_head), head = (int)(vector % p.kv_heads);
-    long long rest = vector / p.kv_heads;
-    const int row = (int)(rest % p.rows);
-    rest /= p.rows;
-    const bool value = rest & 1;
-    const long long site = rest >> 1;
-    const int slot = p.slots[row];
+    const uint32_t per_head = (uint32_t)(p.dim + 7) / 8, at = blockIdx.x * 256 + threadIdx.x;
+    if (at >= p.pieces) return;
+    const uint32_t vector = at / per_head, pair = vector / p.kv_heads, site = blockIdx.y;
+    const int c0 = 8 * (int)(at - vector * per_head), head = (int)(vector - pair * p.kv_heads);
+    const bool value = pair >= (uint32_t)p.rows;                   // (all keys first: a wave does one thing)
+    const int row = (int)(value ? pair - p.rows : pair), slot = p.slots[row];
     uint4 w = make_uint4(0, 0, 0, 0);
     if (slot >= 0 && slot >> p.shift < p.n_pages) {
         const int t = slot & ((1 << p.shift) - 1);
-        const uint8_t* page = p.pages + ((size_t)(site * p.n_pages + (slot >> p.shift)) * p.kv_heads + head) * cache4_record(p.dp, 1 << p.shift);
+        const uint8_t* page = p.pages + (((size_t)site * p.n_pages + (slot >> p.shift)) * p.kv_heads + head) * cache4_record(p.dp, 1 << p.shift);
         uint32_t word = 0;
         const int width = cache4_cut(p.dp) / 16;
         if (!value) word = *(const uint32_t*)(page + cache4_key_at(p.dp, t, c0));
@@ -164,7 +202,7 @@ read4_kernel(Read4Args p) {
         else for (int i = 0; i < 4; ++i) word |= (uint32_t)page[cache4_value_at(p.dp, p.shift, t, c0 + 2 * i)] << (8 * i);
         w = cache4_eight(word, page[cache4_scale_at(p.dp, p.shift, t, c0 / 32, value)]);
     }
-    bf16_t* out = (value ? p.values : p.keys) + ((size_t)(site * p.rows + row) * p.kv_heads + head) * p.dim + c0;
+    bf16_t* out = (value ? p.values : p.keys) + (((size_t)site * p.rows + row) * p.kv_heads + head) * p.dim + c0;
     if (p.dim % 8 == 0) {
         *(uint4*)out = w;
     } else {
@@ -174,10 +212,12 @@ read4_kernel(Read4Args p) {
 }
 
 // Which keys stay: of n the last `recent`, and of those before them the ones with the largest weights, as many as fill `keep`; of equal weights
-// the one that came first.  A block is one head of one request at one site.  The least weight that stays is found digit by digit of eight bits
-// (a float's order is that of its bits, turned round for negative ones; a NaN is the least); then one pass from the front writes the kept
-// indices and weights in order.  Both passes read the weights again from the second-level cache, which holds them.
-// The weights may be moved within their own row: a kept one never moves up, and a piece is read whole before any of it is written.
+// the one that came first.  A block is one head of one request at one site, its weights 16 a thread in registers (longer rows: 16,384 at a time,
+// read again from the second-level cache for every pass).  The least weight that stays is found digit by digit of eight bits, from
+// the first bit in which any two differ: the digits then spread over the counters, where those of whole floats would all meet at a few
+// (a float's order is that of its bits, turned round for negative ones; a NaN is the least).  Then the kept indices and weights go out in
+// order, their places from counts by wave and 1,024: four meetings of the block a 16,384, where one for every 1,024 took 38 us for 16,384 keys.
+// The weights may be moved within their own row: a kept one never moves up, and a 16,384 is read whole before any of it is written.
 struct Evict4Args {
     const int* lengths; const int* slots; const int* new_slots; const int* tables; const int* new_tables;
     uint8_t* pages; int* kept;
@@ -191,17 +231,39 @@ __device__ __forceinline__ uint32_t weight_order(float w) {
     const uint32_t b = __float_as_uint(w == 0.f ? 0.f : w);        // (both zeros are alike)
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float weight_of(uint32_t k) { return k == 0u ? NAN : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-#define EVICT_THREADS 1024
+#define EVICT_HOLD 16
+// The sum of the counts before this wave's in turn j ([turn][wave] order), and of all: by one wave's scan of N counts a lane, read back.
+template <int N>
+__device__ __forceinline__ void evict_scan(int (&counts)[N * WAVE], int tid, int& all) {
+    if (tid < WAVE) {
+        int own[N], sum = 0;
+#pragma unroll
+        for (int j = 0; j < N; ++j) { own[j] = sum; sum += counts[N * tid + j]; }
+        int up = sum;
+#pragma unroll
+        for (int off = 1; off < WAVE; off <<= 1) {
+            const int other = __shfl_up(up, off, WAVE);
+            if (tid >= off) up += other;
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j) counts[N * tid + j] = up - sum + own[j];
+        if (tid == WAVE - 1) all = up;
+    }
+}
+
+template <int EVICT_THREADS>
 __global__ void __launch_bounds__(EVICT_THREADS)
 evict4_select(Evict4Args p) {
-    constexpr int WAVES = EVICT_THREADS / WAVE;
-    __shared__ uint32_t bins[256], below[256];
-    __shared__ uint32_t digit, above;
-    __shared__ int larger[2][WAVES], equal[2][WAVES];
+    constexpr int WAVES = EVICT_THREADS / WAVE, SPAN = EVICT_HOLD * EVICT_THREADS, N = EVICT_HOLD * WAVES / WAVE;
+    static_assert(EVICT_HOLD * WAVES % WAVE == 0, "one wave scans whole counts a lane");
+    __shared__ uint32_t bins[256], ends[2];
+    __shared__ int counts[EVICT_HOLD * WAVES], more[2];
+    __shared__ uint32_t digit, above, here;
     const int head = blockIdx.x % p.kv_heads, request = blockIdx.x / p.kv_heads, site = blockIdx.y, tid = threadIdx.x;
     const int from = p.slots[request], to = p.new_slots[request];
-    int n = min(min(p.lengths[request], p.capacity), p.width << p.shift);
+    int n = (int)min((long long)min(p.lengths[request], p.capacity), (long long)p.width << p.shift);
     if (from < 0 || from >= p.n_slots || to < 0 || to >= p.n_slots) n = 0;
     float* base = p.weights[site];
     const float* w = base + ((size_t)max(from, 0) * p.kv_heads + head) * p.capacity;
@@ -213,15 +275,48 @@ evict4_select(Evict4Args p) {
     }
     const int old = max(0, n - p.recent);                           // these are ranked
     int take = n <= p.keep ? old : p.keep - (n - old);              // and so many of them stay
+    const bool all = take >= old;
+    uint32_t k[EVICT_HOLD];
+    auto load = [&](int i0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < EVICT_HOLD; ++j) {
+            if (i0 + j * EVICT_THREADS >= n) break;
+            const int i = i0 + j * EVICT_THREADS + tid;
+            k[j] = i < n ? weight_order(w[i]) : 0u;
+        }
+    };
+    load(0);
     uint32_t least = 0;                                             // kept: above `least`, and the first `take` at it
-    if (take < old) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
+    if (!all && take > 0) {
+        // the smallest and the largest of the ranked
+        uint32_t low = 0xffffffffu, high = 0u;
+        for (int i0 = 0; i0 < old; i0 += SPAN) {
+            if (i0 > 0) load(i0);
+#pragma unroll
+            for (int j = 0; j < EVICT_HOLD; ++j)
+                if (i0 + j * EVICT_THREADS + tid < old) { low = min(low, k[j]); high = max(high, k[j]); }
+        }
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) { low = min(low, __shfl_xor(low, off, WAVE)); high = max(high, __shfl_xor(high, off, WAVE)); }
+        if (tid == 0) { ends[0] = 0xffffffffu; ends[1] = 0u; }
+        __syncthreads();
+        if (tid % WAVE == 0) { atomicMin(&ends[0], low); atomicMax(&ends[1], high); }
+        __syncthreads();
+        low = ends[0];
+        high = ends[1];
+        least = low;                                                // (the digits found so far, from `low` on)
+        int bits = high > low ? 32 - __clz(high - low) : 0;         // that are still open
+        while (bits > 0) {
+            const int shift = max(bits - 8, 0);
             if (tid < 256) bins[tid] = 0;
             __syncthreads();
-            const uint32_t mask = shift == 24 ? 0u : ~0u << (shift + 8);
-            for (int i = tid; i < old; i += EVICT_THREADS) {
-                const uint32_t k = weight_order(w[i]);
-                if ((k & mask) == least) atomicAdd(&bins[(k >> shift) & 255], 1u);
+            for (int i0 = 0; i0 < old; i0 += SPAN) {
+                if (old > SPAN) load(i0);
+#pragma unroll
+                for (int j = 0; j < EVICT_HOLD; ++j) {
+                    const uint32_t d = k[j] - least;                // (below `least`: a large number)
+                    if (i0 + j * EVICT_THREADS + tid < old && k[j] >= least && (bits == 32 || d >> bits == 0)) atomicAdd(&bins[d >> shift], 1u);
+                }
             }
             __syncthreads();
             // entries of a larger digit, by a sum from the top over one wave: four digits a lane
@@ -238,93 +333,140 @@ evict4_select(Evict4Args p) {
                 over -= sum;                                        // of the lanes above
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint32_t more = over + own[j], here = bins[4 * tid + j];
-                    if (more < (uint32_t)take && more + here >= (uint32_t)take) { digit = 4 * tid + j; above = more; }
+                    const uint32_t larger = over + own[j], equal = bins[4 * tid + j];
+                    if (larger < (uint32_t)take && larger + equal >= (uint32_t)take) { digit = 4 * tid + j; above = larger; here = equal; }
                 }
-                if (tid == 0 && take <= 0) { digit = 255; above = 0; }
             }
             __syncthreads();
-            least |= digit << shift;
+            least += digit << shift;
             take -= (int)above;
+            bits = shift;
+            const bool whole = (int)here == take;                   // all of this digit stay: the rest of the bits say nothing
             __syncthreads();
+            if (whole) {
+                take = 0x7fffffff;
+                break;
+            }
         }
-    } else {
+        if (old > SPAN) load(0);
+    } else if (!all) {
+        least = 0xffffffffu;
         take = 0;
     }
-    const bool all = n <= p.keep || p.keep - (n - old) >= old;
-    // (of those at `least` the first `take` stay)
     const int lane = tid % WAVE, wave = tid / WAVE;
-    int done = 0, met = 0, turn = 0;
-    for (int i0 = 0; i0 < n; i0 += EVICT_THREADS, turn ^= 1) {
-        const int i = i0 + tid;
-        const float weight = i < n ? w[i] : 0.f;
-        const uint32_t k = weight_order(weight);
-        const bool ranked = i < old && !all;
-        const bool tie = ranked && k == least;
-        const unsigned long long ties = __ballot(tie);
-        if (lane == 0) equal[turn][wave] = __popcll(ties);
-        __syncthreads();                                            // (and everyone has read its weight)
-        int tied = met + __popcll(ties & ((1ull << lane) - 1)), ties_all = 0;
+    int done = 0, met = 0;
+    for (int i0 = 0; i0 < n; i0 += SPAN) {
+        if (i0 > 0) load(i0);
+        unsigned long long tie[EVICT_HOLD];
 #pragma unroll
-        for (int v = 0; v < WAVES; ++v) { const int e = equal[turn][v]; tied += v < wave ? e : 0; ties_all += e; }
-        const bool stays = i < n && (!ranked || k > least || (tie && tied < take));
-        const unsigned long long stay = __ballot(stays);
-        if (lane == 0) larger[turn][wave] = __popcll(stay);
+        for (int j = 0; j < EVICT_HOLD; ++j) {
+            tie[j] = __ballot(!all && i0 + j * EVICT_THREADS + tid < old && k[j] == least);
+            if (lane == 0) counts[j * WAVES + wave] = __popcll(tie[j]);
+        }
+        __syncthreads();                                            // (and everyone has read its weights)
+        evict_scan<N>(counts, tid, more[0]);
         __syncthreads();
-        int to_index = done + __popcll(stay & ((1ull << lane) - 1)), all_stay = 0;
+        unsigned long long stay[EVICT_HOLD];
 #pragma unroll
-        for (int v = 0; v < WAVES; ++v) { const int e = larger[turn][v]; to_index += v < wave ? e : 0; all_stay += e; }
-        if (stays && to_index < p.keep) { kept[to_index] = i; nw[to_index] = weight; }
-        done += all_stay;
-        met += ties_all;
+        for (int j = 0; j < EVICT_HOLD; ++j) {
+            const int i = i0 + j * EVICT_THREADS + tid, tied = met + counts[j * WAVES + wave] + __popcll(tie[j] & ((1ull << lane) - 1));
+            stay[j] = __ballot(i < n && (all || i >= old || k[j] > least || (k[j] == least && tied < take)));
+        }
+        met += more[0];
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < EVICT_HOLD; ++j) if (lane == 0) counts[j * WAVES + wave] = __popcll(stay[j]);
+        __syncthreads();
+        evict_scan<N>(counts, tid, more[1]);
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < EVICT_HOLD; ++j) {
+            const int place = done + counts[j * WAVES + wave] + __popcll(stay[j] & ((1ull << lane) - 1));
+            if (stay[j] >> lane & 1 && place < p.keep) { kept[place] = i0 + j * EVICT_THREADS + tid; nw[place] = weight_of(k[j]); }
+        }
+        done += more[1];
+        __syncthreads();
     }
-    __syncthreads();
     const int m = min(done, p.keep);
     for (int i = m + tid; i < p.keep; i += EVICT_THREADS) kept[i] = -1;
     for (int i = m + tid; i < p.capacity; i += EVICT_THREADS) nw[i] = 0.f;
 }
 
-// The kept keys and values, from the pages that held them to the pages of the new table: a block is eight tokens of a head.
+// The kept keys and values, from the pages that held them to the pages of the new table: a block is 64 tokens of a head.  Keys go in rows of 16-byte
+// pieces; of the values a thread gathers the run of a column and eight tokens and writes it whole, likewise of the scales.
+#define EVICT_TOKENS 64
 __global__ void __launch_bounds__(256)
 evict4_move(Evict4Args p) {
-    const int eights = (p.keep + 7) / 8, tid = threadIdx.x;
-    const int eight = blockIdx.x % eights, head = blockIdx.x / eights, request = blockIdx.y, site = blockIdx.z;
-    const int P = 1 << p.shift, record = cache4_record(p.dp, P), first = 8 * eight;
-    __shared__ const uint8_t* source[8];
-    __shared__ int token[8];
+    const int tiles = (p.keep + EVICT_TOKENS - 1) / EVICT_TOKENS, tid = threadIdx.x;
+    const int tile = blockIdx.x % tiles, head = blockIdx.x / tiles, request = blockIdx.y, site = blockIdx.z;
+    const int P = 1 << p.shift, mask = P - 1, record = cache4_record(p.dp, P), first = EVICT_TOKENS * tile;
+    __shared__ const uint8_t* source[EVICT_TOKENS];                 // of a token: its page, and the page of its place; null where there is none
+    __shared__ uint8_t* target[EVICT_TOKENS];
+    __shared__ int token[EVICT_TOKENS];
     const int* kept = p.kept + (((size_t)site * p.requests + request) * p.kv_heads + head) * p.keep;
-    uint8_t* site_pages = p.pages + (size_t)site * p.n_pages * p.kv_heads * record;
-    const int to = first >> p.shift < p.new_width ? p.new_tables[(size_t)request * p.new_width + (first >> p.shift)] : -1;
-    if (tid < 8) {
-        const int k = first + tid < p.keep ? kept[first + tid] : -1;
-        const int page = k >= 0 ? p.tables[(size_t)request * p.width + (k >> p.shift)] : -1;
-        source[tid] = page >= 0 && page < p.n_pages ? site_pages + ((size_t)page * p.kv_heads + head) * record : nullptr;
-        token[tid] = k & (P - 1);
+    uint8_t* pages = p.pages + (size_t)site * p.n_pages * p.kv_heads * record;
+    if (tid < EVICT_TOKENS) {
+        const int i = first + tid, k = i < p.keep ? kept[i] : -1;
+        const int page = k >= 0 && k >> p.shift < p.width ? p.tables[(size_t)request * p.width + (k >> p.shift)] : -1;
+        const int to = i >> p.shift < p.new_width ? p.new_tables[(size_t)request * p.new_width + (i >> p.shift)] : -1;
+        source[tid] = page >= 0 && page < p.n_pages ? pages + ((size_t)page * p.kv_heads + head) * record : nullptr;
+        target[tid] = to >= 0 && to < p.n_pages ? pages + ((size_t)to * p.kv_heads + head) * record : nullptr;
+        token[tid] = k & mask;
     }
     __syncthreads();
-    if (to < 0 || to >= p.n_pages) return;
-    uint8_t* target = site_pages + ((size_t)to * p.kv_heads + head) * record;
-    const int words = p.dp / 8, w = cache4_cut(p.dp) / 16;          // 4-byte words a token's key
-    for (int i = tid; i < 8 * words; i += 256) {
-        const int t = i / words, x = i % words;
-        if (source[t]) *(uint32_t*)(target + ((first & (P - 1)) + t) * (p.dp / 2) + 4 * x) = *(const uint32_t*)(source[t] + token[t] * (p.dp / 2) + 4 * x);
+    const int pieces = p.dp / 32;
+    for (int i = tid; i < EVICT_TOKENS * pieces; i += 256) {
+        const int t = i / pieces, x = i - t * pieces;
+        if (source[t] && target[t]) *(uint4*)(target[t] + ((first + t) & mask) * (p.dp / 2) + 16 * x) = *(const uint4*)(source[t] + token[t] * (p.dp / 2) + 16 * x);
     }
-    // values: pieces of w / 2 bytes, the eight tokens side by side
-    const int pieces = p.dp / w;
-    for (int i = tid; i < 8 * pieces; i += 256) {
-        const int t = i & 7, d = (i >> 3) * w;
-        if (!source[t]) continue;
-        uint8_t* out = target + cache4_value_at(p.dp, p.shift, (first & (P - 1)) + t, d);
-        const uint8_t* in = source[t] + cache4_value_at(p.dp, p.shift, token[t], d);
-        if (w == 8) *(uint32_t*)out = *(const uint32_t*)in;
-        else if (w == 4) *(uint16_t*)out = *(const uint16_t*)in;
-        else *out = *in;
+    const int cut = cache4_cut(p.dp), w = cut / 16, columns = p.dp / w;
+    for (int i = tid; i < EVICT_TOKENS / 8 * columns; i += 256) {
+        const int e = i / columns, d = (i - e * columns) * w, t0 = 8 * e;
+        if (!target[t0]) continue;                                  // (eight tokens are in one page)
+        uint8_t* out = target[t0] + cache4_value_at(p.dp, p.shift, (first + t0) & mask, d);
+        bool whole = true;
+        uint32_t run[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            const uint8_t* in = source[t0 + t] ? source[t0 + t] + cache4_value_at(p.dp, p.shift, token[t0 + t], d) : nullptr;
+            whole &= in != nullptr;
+            run[t] = !in ? 0u : w == 8 ? *(const uint32_t*)in : w == 4 ? *(const uint16_t*)in : *in;
+        }
+        if (whole && w == 8) {
+            *(uint4*)out = make_uint4(run[0], run[1], run[2], run[3]);
+            *(uint4*)(out + 16) = make_uint4(run[4], run[5], run[6], run[7]);
+        } else if (whole && w == 4) {
+            *(uint4*)out = make_uint4(run[0] | run[1] << 16, run[2] | run[3] << 16, run[4] | run[5] << 16, run[6] | run[7] << 16);
+        } else if (whole) {
+            *(uint2*)out = make_uint2(run[0] | run[1] << 8 | run[2] << 16 | run[3] << 24, run[4] | run[5] << 8 | run[6] << 16 | run[7] << 24);
+        } else {                                                    // (what lies behind the last kept key is left as it is)
+#pragma unroll
+            for (int t = 0; t < 8; ++t)
+                if (source[t0 + t]) {
+                    if (w == 8) *(uint32_t*)(out + 4 * t) = run[t];
+                    else if (w == 4) *(uint16_t*)(out + 2 * t) = (uint16_t)run[t];
+                    else out[t] = (uint8_t)run[t];
+                }
+        }
     }
-    const int scales = 2 * (p.dp / 32);
-    for (int i = tid; i < 8 * scales; i += 256) {
-        const int t = i & 7, b = i >> 3, blocks = p.dp / 32;
-        if (source[t])
-            target[cache4_scale_at(p.dp, p.shift, (first & (P - 1)) + t, b % blocks, b >= blocks)] = source[t][cache4_scale_at(p.dp, p.shift, token[t], b % blocks, b >= blocks)];
+    const int blocks = p.dp / 32;
+    for (int i = tid; i < EVICT_TOKENS / 8 * 2 * blocks; i += 256) {
+        const int e = i / (2 * blocks), b = i - e * 2 * blocks, t0 = 8 * e;
+        if (!target[t0]) continue;
+        const bool value = b >= blocks;
+        bool whole = true;
+        uint8_t* out = target[t0] + cache4_scale_at(p.dp, p.shift, (first + t0) & mask, value ? b - blocks : b, value);
+        uint32_t run[8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t) whole &= source[t0 + t] != nullptr;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) run[t] = source[t0 + t] ? source[t0 + t][cache4_scale_at(p.dp, p.shift, token[t0 + t], value ? b - blocks : b, value)] : 0u;
+        if (whole) {
+            *(uint2*)out = make_uint2(run[0] | run[1] << 8 | run[2] << 16 | run[3] << 24, run[4] | run[5] << 8 | run[6] << 16 | run[7] << 24);
+        } else {
+#pragma unroll
+            for (int t = 0; t < 8; ++t) if (source[t0 + t]) out[t] = (uint8_t)run[t];
+        }
     }
 }
 
@@ -371,10 +513,14 @@ int cisr_write4(const void* qkv, const int* positions, const int* slots, const f
     const int dp = (dim + 31) / 32 * 32;
     Write4Args p = {qkv, positions, slots, cos, sin, (uint8_t*)pages, q, rows, heads, kv_heads, dim, dp, rot, __builtin_ctz(page), max_pos, n_pages, interleaved};
     const long long blocks = ((long long)rows * (heads + 2 * kv_heads) * (dp / 8) + 255) / 256;
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+    if (blocks > INT32_MAX / 256) return hipErrorInvalidValue;
     const uintptr_t both = (uintptr_t)qkv | (uintptr_t)q | (uintptr_t)cos | (uintptr_t)sin;
     const bool words = !interleaved && dim % 8 == 0 && rot % 16 == 0 && both % 16 == 0;
-    if (dtype == DT_BF16) {
+    if (words && rot == dim && dim % 64 == 0) {
+        const int half_blocks = (int)(((long long)rows * (heads + 2 * kv_heads) * (dim / 16) + 255) / 256);
+        if (dtype == DT_BF16) write4_halves_kernel<bf16_t><<<half_blocks, 256, 0, (hipStream_t)stream>>>(p);
+        else write4_halves_kernel<float><<<half_blocks, 256, 0, (hipStream_t)stream>>>(p);
+    } else if (dtype == DT_BF16) {
         if (words) write4_kernel<bf16_t, true><<<(int)blocks, 256, 0, (hipStream_t)stream>>>(p);
         else write4_kernel<bf16_t, false><<<(int)blocks, 256, 0, (hipStream_t)stream>>>(p);
     } else {
@@ -386,11 +532,10 @@ int cisr_write4(const void* qkv, const int* positions, const int* slots, const f
 
 int cisr_read4(const void* pages, const int* slots, void* keys, void* values, int sites, int rows, int kv_heads, int dim, int page, int n_pages, void* stream) {
     if (sites <= 0 || rows <= 0 || kv_heads <= 0 || dim <= 0 || dim > 256 || dim % 2 || page < 8 || (page & (page - 1)) || n_pages <= 0) return hipErrorInvalidValue;
-    Read4Args p = {(const uint8_t*)pages, slots, (bf16_t*)keys, (bf16_t*)values, (long long)sites * rows * kv_heads * 2, rows, kv_heads, dim, (dim + 31) / 32 * 32,
-                   __builtin_ctz(page), n_pages};
-    const long long blocks = (p.vectors * ((dim + 7) / 8) + 255) / 256;
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;
-    read4_kernel<<<(int)blocks, 256, 0, (hipStream_t)stream>>>(p);
+    const long long pieces = (long long)rows * kv_heads * 2 * ((dim + 7) / 8);
+    if (pieces > INT32_MAX || sites > 65535) return hipErrorInvalidValue;
+    Read4Args p = {(const uint8_t*)pages, slots, (bf16_t*)keys, (bf16_t*)values, (uint32_t)pieces, rows, kv_heads, dim, (dim + 31) / 32 * 32, __builtin_ctz(page), n_pages};
+    read4_kernel<<<dim3((uint32_t)((pieces + 255) / 256), sites), 256, 0, (hipStream_t)stream>>>(p);
     return hipGetLastError();
 }
 
@@ -406,10 +551,12 @@ int cisr_evict4(const int* lengths, const int* slots, const int* new_slots, cons
         Evict4Args p = {lengths, slots, new_slots, tables, new_tables, (uint8_t*)pages + at * site_bytes, kept + (size_t)at * requests * kv_heads * keep, n_pages,
                         requests, kv_heads, dp, __builtin_ctz(page), width, new_width, keep, recent, capacity, n_slots, now, {}};
         for (int s = 0; s < now; ++s) p.weights[s] = (float*)weights[at + s];
-        evict4_select<<<dim3(requests * kv_heads, now), EVICT_THREADS, 0, (hipStream_t)stream>>>(p);
+        // (blocks of four waves meet faster, and hold rows of up to 4,096)
+        if ((capacity < (long long)width * page ? capacity : (long long)width * page) <= 256 * EVICT_HOLD) evict4_select<256><<<dim3(requests * kv_heads, now), 256, 0, (hipStream_t)stream>>>(p);
+        else evict4_select<1024><<<dim3(requests * kv_heads, now), 1024, 0, (hipStream_t)stream>>>(p);
         hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
-        evict4_move<<<dim3((keep + 7) / 8 * kv_heads, requests, now), 256, 0, (hipStream_t)stream>>>(p);
+        evict4_move<<<dim3((keep + EVICT_TOKENS - 1) / EVICT_TOKENS * kv_heads, requests, now), 256, 0, (hipStream_t)stream>>>(p);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
     }

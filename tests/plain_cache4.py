@@ -113,6 +113,6 @@ def stays(w, n, keep, recent):
     if n <= keep:
         return list(range(n))
     old = max(0, n - recent)
-    value = [(-math.inf if math.isnan(float(x)) else float(x)) for x in w[:old]]
-    order = sorted(range(old), key=lambda i: (-value[i], i))
+    value = [float(x) for x in w[:old]]
+    order = sorted(range(old), key=lambda i: (math.isnan(value[i]), 0.0 if math.isnan(value[i]) else -value[i], i))      # (a NaN is below every number)
     return sorted(order[:keep - (n - old)]) + list(range(old, n))

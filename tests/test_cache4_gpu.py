@@ -285,3 +285,34 @@ def test_evict_many_keys_and_sites():
         assert torch.equal(sums[site][0, 0, :keep].cpu(), before[site][0, 0, index]) and not sums[site][0, 0, keep:].any()
         c.read(storage[site:site + 1], torch.tensor(index, dtype=torch.int32, device=GPU), ka[:1], vb[:1], kv, dim, P)
         assert torch.equal(a[site], ka[0]) and torch.equal(b[site], vb[0])
+
+
+@pytest.mark.parametrize("n,keep,recent", [(40000, 3000, 100), (40000, 39000, 0), (16385, 16384, 16000), (16384, 1, 0), (33000, 20000, 20000)])
+@pytest.mark.parametrize("kind", ["spread", "ties", "alike", "narrow", "special"])
+def test_which_keys_stay_of_long_rows(n, keep, recent, kind):
+    """Rows past what a block holds in registers; sums that are all alike, differ in a few last bits, or are no numbers."""
+    c, g = cache4(), torch.Generator().manual_seed(n + keep)
+    w = torch.exp(4 * torch.randn(2, n, generator=g))
+    if kind == "ties":
+        w = (torch.rand(2, n, generator=g) * 5).round()
+    elif kind == "alike":
+        w = torch.full((2, n), 3.0)
+    elif kind == "narrow":
+        w = (torch.full((2, n), 1.0).view(torch.int32) + torch.randint(0, 5, (2, n), generator=g, dtype=torch.int32)).view(torch.float32)
+    elif kind == "special":
+        w = torch.tensor([math.nan, math.inf, -math.inf, 0.0, -0.0, 1e-45, -1.0, 3e38])[torch.randint(0, 8, (2, n), generator=g)]
+    P, dim = 16, 32
+    pages = -(-n // P) + -(-keep // P)
+    storage = torch.zeros(1, pages, 2, c.record_bytes(dim, P), dtype=torch.uint8, device=GPU)
+    sums = [w[None].clone().to(GPU)]
+    tables = torch.arange(-(-n // P), device=GPU, dtype=torch.int32)[None]
+    new_tables = torch.arange(-(-n // P), pages, device=GPU, dtype=torch.int32)[None]
+    kept = torch.empty(1, 1, 2, keep, dtype=torch.int32, device=GPU)
+    zero = torch.zeros(1, dtype=torch.int32, device=GPU)
+    c.evict(storage, sums, tables, new_tables, zero + n, zero, zero, 2, dim, P, keep, recent, kept)
+    for h in range(2):
+        index = plain.stays(w[h].tolist(), n, keep, recent)
+        assert kept[0, 0, h].tolist() == index
+        want = torch.zeros(n)
+        want[:keep] = w[h, index]
+        assert torch.equal(torch.nan_to_num(sums[0][0, h].cpu(), nan=-5.0), torch.nan_to_num(want, nan=-5.0))
