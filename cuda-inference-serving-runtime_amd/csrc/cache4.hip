@@ -487,15 +487,31 @@ merge4_kernel(Merge4Args p) {
     if (item >= rows * p.heads) return;
     const int r = item / p.heads, h = item - r * p.heads, kvh = h / p.group;
     const size_t one = ((size_t)kvh * p.rows_per_task + r) * p.group + h - kvh * p.group, step = (size_t)p.heads * p.rows_per_task;
+    // (eight pieces' loads are on their way together: one trip to memory instead of one a piece)
     float m = CACHE4_NOTHING, l = 0.f, a = 0.f, b = 0.f;
-    for (int s = 0; s < pieces; ++s) {
-        const size_t part = (first + s) * step + one;
-        const float2 ml = *(const float2*)(p.part_ml + 2 * part), v = *(const float2*)(p.part_o + part * p.dim + d);
-        const float top = fmaxf(m, ml.x), f = exp2f(m - top), g = exp2f(ml.x - top);
+    for (int s0 = 0; s0 < pieces; s0 += 8) {
+        float2 ml[8], v[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            const size_t part = (first + min(s0 + s, pieces - 1)) * step + one;
+            ml[s] = *(const float2*)(p.part_ml + 2 * part);
+            v[s] = *(const float2*)(p.part_o + part * p.dim + d);
+        }
+        float top = m;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) top = s0 + s < pieces ? fmaxf(top, ml[s].x) : top;
+        const float f = exp2f(m - top);
         m = top;
-        l = fmaf(ml.y, g, l * f);
-        a = fmaf(v.x, g, a * f);
-        b = fmaf(v.y, g, b * f);
+        l *= f;
+        a *= f;
+        b *= f;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            const float g = s0 + s < pieces ? exp2f(ml[s].x - top) : 0.f;
+            l = fmaf(ml[s].y, g, l);
+            a = fmaf(v[s].x, g, a);
+            b = fmaf(v[s].y, g, b);
+        }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const size_t to = (size_t)(row0 + r) * p.heads + h;
