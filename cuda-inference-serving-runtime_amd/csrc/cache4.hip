@@ -216,7 +216,9 @@ read4_kernel(Read4Args p) {
 // read again from the second-level cache for every pass).  The least weight that stays is found digit by digit of eight bits, from
 // the first bit in which any two differ: the digits then spread over the counters, where those of whole floats would all meet at a few
 // (a float's order is that of its bits, turned round for negative ones; a NaN is the least).  Then the kept indices and weights go out in
-// order, their places from counts by wave and 1,024: four meetings of the block a 16,384, where one for every 1,024 took 38 us for 16,384 keys.
+// order, their places from counts by wave and turn.  What the block has to agree on is found by every wave for itself from counters in LDS, so that a pass and
+// a 16,384 cost one meeting each.  Bound by that chain: 14 us for 90 heads of 2,112 keys, 21 for 128 of up to 16,384 (18 and 26 with four meetings a pass,
+// one counter a digit and a branch round each load).
 // The weights may be moved within their own row: a kept one never moves up, and a 16,384 is read whole before any of it is written.
 struct Evict4Args {
     const int* lengths; const int* slots; const int* new_slots; const int* tables; const int* new_tables;
@@ -234,34 +236,51 @@ __device__ __forceinline__ uint32_t weight_order(float w) {
 __device__ __forceinline__ float weight_of(uint32_t k) { return k == 0u ? NAN : __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 #define EVICT_HOLD 16
-// The sum of the counts before this wave's in turn j ([turn][wave] order), and of all: by one wave's scan of N counts a lane, read back.
-template <int N>
-__device__ __forceinline__ void evict_scan(int (&counts)[N * WAVE], int tid, int& all) {
-    if (tid < WAVE) {
-        int own[N], sum = 0;
+#define EVICT_COPIES 4
+// The sum over this lane and those below it, without LDS: within rows of 16 lanes, then over the rows.
+__device__ __forceinline__ uint32_t wave_prefix(uint32_t x) {
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xf, 0xf, true);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xf, 0xf, true);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xf, 0xf, true);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xf, 0xf, true);
+    x += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xa, 0xf, false);
+    return x + (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x143, 0xc, 0xf, false);
+}
+// How many lanes below this one are set.
+__device__ __forceinline__ int lanes_below(unsigned long long set) {
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(set >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)set, 0u));
+}
+// Digits' counts of one pass as each wave takes them (four a lane): the digit whose entries reach `take` from the top, how many are of larger ones, how many its own.
+struct EvictDigit { uint32_t digit, above, here; };
+__device__ __forceinline__ EvictDigit evict_digit(const uint32_t (&bins)[256 * EVICT_COPIES], int lane, uint32_t take) {
+    uint4 of;
+    uint32_t* each = &of.x;
 #pragma unroll
-        for (int j = 0; j < N; ++j) { own[j] = sum; sum += counts[N * tid + j]; }
-        int up = sum;
-#pragma unroll
-        for (int off = 1; off < WAVE; off <<= 1) {
-            const int other = __shfl_up(up, off, WAVE);
-            if (tid >= off) up += other;
-        }
-#pragma unroll
-        for (int j = 0; j < N; ++j) counts[N * tid + j] = up - sum + own[j];
-        if (tid == WAVE - 1) all = up;
+    for (int j = 0; j < 4; ++j) {
+        const uint4 x = *(const uint4*)&bins[EVICT_COPIES * (4 * lane + j)];
+        each[j] = x.x + x.y + x.z + x.w;
     }
+    const uint32_t sum = of.x + of.y + of.z + of.w, up = wave_prefix(sum);
+    const uint32_t over = (uint32_t)__builtin_amdgcn_readlane((int)up, WAVE - 1) - up + sum;      // of this lane's digits and larger ones
+    uint32_t larger = over - sum, j = 3, here = of.w;
+    if (larger + of.w < take) { larger += of.w; j = 2; here = of.z;
+        if (larger + of.z < take) { larger += of.z; j = 1; here = of.y;
+            if (larger + of.y < take) { larger += of.y; j = 0; here = of.x; } } }
+    const int owner = __ffsll(__ballot(over >= take && over - sum < take)) - 1;      // (one lane: 0 < take <= all entries)
+    return {(uint32_t)__builtin_amdgcn_readlane((int)(4 * lane + j), owner), (uint32_t)__builtin_amdgcn_readlane((int)larger, owner),
+            (uint32_t)__builtin_amdgcn_readlane((int)here, owner)};
 }
 
 template <int EVICT_THREADS>
 __global__ void __launch_bounds__(EVICT_THREADS)
 evict4_select(Evict4Args p) {
     constexpr int WAVES = EVICT_THREADS / WAVE, SPAN = EVICT_HOLD * EVICT_THREADS, N = EVICT_HOLD * WAVES / WAVE;
-    static_assert(EVICT_HOLD * WAVES % WAVE == 0, "one wave scans whole counts a lane");
-    __shared__ uint32_t bins[256], ends[2];
-    __shared__ int counts[EVICT_HOLD * WAVES], more[2];
-    __shared__ uint32_t digit, above, here;
+    static_assert(N == 1 || N == 4, "a wave takes all counts, one or four a lane");
+    __shared__ __attribute__((aligned(16))) uint32_t bins[4][256 * EVICT_COPIES];
+    __shared__ uint32_t ends[2][WAVES];               // (a pass has its own counters: no meeting to clear them; four for each digit, as most entries share a few)
+    __shared__ __attribute__((aligned(16))) uint32_t counts[2][EVICT_HOLD * WAVES];              // [turn][wave]: entries above `least`, and 65,536 times those at it
     const int head = blockIdx.x % p.kv_heads, request = blockIdx.x / p.kv_heads, site = blockIdx.y, tid = threadIdx.x;
+    const int lane = tid % WAVE, wave = __builtin_amdgcn_readfirstlane(tid / WAVE);
     const int from = p.slots[request], to = p.new_slots[request];
     int n = (int)min((long long)min(p.lengths[request], p.capacity), (long long)p.width << p.shift);
     if (from < 0 || from >= p.n_slots || to < 0 || to >= p.n_slots) n = 0;
@@ -280,10 +299,11 @@ evict4_select(Evict4Args p) {
     auto load = [&](int i0) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < EVICT_HOLD; ++j) {
-            if (i0 + j * EVICT_THREADS >= n) break;
             const int i = i0 + j * EVICT_THREADS + tid;
-            k[j] = i < n ? weight_order(w[i]) : 0u;
+            k[j] = __float_as_uint(w[min(i, n - 1)]);               // (no branch round a load: all are on their way together)
         }
+#pragma unroll
+        for (int j = 0; j < EVICT_HOLD; ++j) k[j] = weight_order(__uint_as_float(k[j]));
     };
     load(0);
     uint32_t least = 0;                                             // kept: above `least`, and the first `take` at it
@@ -298,52 +318,30 @@ evict4_select(Evict4Args p) {
         }
 #pragma unroll
         for (int off = 32; off > 0; off >>= 1) { low = min(low, __shfl_xor(low, off, WAVE)); high = max(high, __shfl_xor(high, off, WAVE)); }
-        if (tid == 0) { ends[0] = 0xffffffffu; ends[1] = 0u; }
+        if (lane == 0) { ends[0][wave] = low; ends[1][wave] = high; }
+        for (int i = tid; i < 256 * EVICT_COPIES; i += EVICT_THREADS) ((uint4*)bins)[i] = make_uint4(0u, 0u, 0u, 0u);
         __syncthreads();
-        if (tid % WAVE == 0) { atomicMin(&ends[0], low); atomicMax(&ends[1], high); }
-        __syncthreads();
-        low = ends[0];
-        high = ends[1];
+#pragma unroll
+        for (int v = 0; v < WAVES; ++v) { low = min(low, ends[0][v]); high = max(high, ends[1][v]); }
         least = low;                                                // (the digits found so far, from `low` on)
         int bits = high > low ? 32 - __clz(high - low) : 0;         // that are still open
-        while (bits > 0) {
+        for (int pass = 0; bits > 0; ++pass) {                      // (four at most: 32 bits in eights)
             const int shift = max(bits - 8, 0);
-            if (tid < 256) bins[tid] = 0;
-            __syncthreads();
             for (int i0 = 0; i0 < old; i0 += SPAN) {
                 if (old > SPAN) load(i0);
 #pragma unroll
                 for (int j = 0; j < EVICT_HOLD; ++j) {
+                    if (i0 + j * EVICT_THREADS >= old) break;
                     const uint32_t d = k[j] - least;                // (below `least`: a large number)
-                    if (i0 + j * EVICT_THREADS + tid < old && k[j] >= least && (bits == 32 || d >> bits == 0)) atomicAdd(&bins[d >> shift], 1u);
+                    if (i0 + j * EVICT_THREADS + tid < old && k[j] >= least && (bits == 32 || d >> bits == 0)) atomicAdd(&bins[pass][EVICT_COPIES * (d >> shift) + lane % EVICT_COPIES], 1u);
                 }
             }
             __syncthreads();
-            // entries of a larger digit, by a sum from the top over one wave: four digits a lane
-            if (tid < WAVE) {
-                uint32_t own[4], sum = 0;
-#pragma unroll
-                for (int j = 3; j >= 0; --j) { own[j] = sum; sum += bins[4 * tid + j]; }
-                uint32_t over = sum;
-#pragma unroll
-                for (int off = 1; off < WAVE; off <<= 1) {
-                    const uint32_t up = __shfl_down(over, off, WAVE);
-                    if (tid + off < WAVE) over += up;
-                }
-                over -= sum;                                        // of the lanes above
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t larger = over + own[j], equal = bins[4 * tid + j];
-                    if (larger < (uint32_t)take && larger + equal >= (uint32_t)take) { digit = 4 * tid + j; above = larger; here = equal; }
-                }
-            }
-            __syncthreads();
-            least += digit << shift;
-            take -= (int)above;
+            const EvictDigit got = evict_digit(bins[pass], lane, (uint32_t)take);
+            least += got.digit << shift;
+            take -= (int)got.above;
             bits = shift;
-            const bool whole = (int)here == take;                   // all of this digit stay: the rest of the bits say nothing
-            __syncthreads();
-            if (whole) {
+            if ((int)got.here == take) {                            // all of this digit stay: the rest of the bits say nothing
                 take = 0x7fffffff;
                 break;
             }
@@ -353,41 +351,49 @@ evict4_select(Evict4Args p) {
         least = 0xffffffffu;
         take = 0;
     }
-    const int lane = tid % WAVE, wave = tid / WAVE;
-    int done = 0, met = 0;
-    for (int i0 = 0; i0 < n; i0 += SPAN) {
+    int done = 0, met = 0;                                          // entries above and at `least` of the spans before
+    for (int i0 = 0, turn = 0; i0 < n; i0 += SPAN, turn ^= 1) {
         if (i0 > 0) load(i0);
-        unsigned long long tie[EVICT_HOLD];
+        unsigned long long tie[EVICT_HOLD], over[EVICT_HOLD];
+        uint32_t mine = 0;
 #pragma unroll
         for (int j = 0; j < EVICT_HOLD; ++j) {
-            tie[j] = __ballot(!all && i0 + j * EVICT_THREADS + tid < old && k[j] == least);
-            if (lane == 0) counts[j * WAVES + wave] = __popcll(tie[j]);
+            const int i = i0 + j * EVICT_THREADS + tid;
+            tie[j] = __ballot(!all && i < old && k[j] == least);
+            over[j] = __ballot(i < n && (all || i >= old || k[j] > least));
+            const uint32_t of = (uint32_t)(__popcll(over[j]) | __popcll(tie[j]) << 16);
+            mine = lane == j ? of : mine;
         }
+        if (lane < EVICT_HOLD) counts[turn][lane * WAVES + wave] = mine;
         __syncthreads();                                            // (and everyone has read its weights)
-        evict_scan<N>(counts, tid, more[0]);
-        __syncthreads();
-        unsigned long long stay[EVICT_HOLD];
+        uint32_t own[N], sum = 0;                                   // (a span has 16,384 entries: neither half runs over)
+        if constexpr (N == 4) {
+            const uint4 x = *(const uint4*)&counts[turn][4 * lane];
+            own[0] = x.x; own[1] = x.y; own[2] = x.z; own[3] = x.w;
+        } else {
+            own[0] = counts[turn][lane];
+        }
+#pragma unroll
+        for (int x = 0; x < N; ++x) { const uint32_t of = own[x]; own[x] = sum; sum += of; }
+        uint32_t up = wave_prefix(sum);
+        const uint32_t total = (uint32_t)__builtin_amdgcn_readlane((int)up, WAVE - 1);
+        up -= sum;
+        uint32_t at = own[0];                                       // before this wave's entry of the lane's N
+#pragma unroll
+        for (int x = 1; x < N; ++x) at = wave % N == x ? own[x] : at;
+        at += up;
 #pragma unroll
         for (int j = 0; j < EVICT_HOLD; ++j) {
-            const int i = i0 + j * EVICT_THREADS + tid, tied = met + counts[j * WAVES + wave] + __popcll(tie[j] & ((1ull << lane) - 1));
-            stay[j] = __ballot(i < n && (all || i >= old || k[j] > least || (k[j] == least && tied < take)));
+            if (i0 + j * EVICT_THREADS >= n) break;
+            const uint32_t first = (uint32_t)__builtin_amdgcn_readlane((int)at, (j * WAVES + wave) / N);
+            const int ties = met + (int)(first >> 16) + lanes_below(tie[j]);
+            const int place = done + (int)(first & 0xffffu) + lanes_below(over[j]) + min(ties, take);
+            if ((over[j] >> lane & 1 || (tie[j] >> lane & 1 && ties < take)) && place < p.keep) { kept[place] = i0 + j * EVICT_THREADS + tid; nw[place] = weight_of(k[j]); }
         }
-        met += more[0];
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < EVICT_HOLD; ++j) if (lane == 0) counts[j * WAVES + wave] = __popcll(stay[j]);
-        __syncthreads();
-        evict_scan<N>(counts, tid, more[1]);
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < EVICT_HOLD; ++j) {
-            const int place = done + counts[j * WAVES + wave] + __popcll(stay[j] & ((1ull << lane) - 1));
-            if (stay[j] >> lane & 1 && place < p.keep) { kept[place] = i0 + j * EVICT_THREADS + tid; nw[place] = weight_of(k[j]); }
-        }
-        done += more[1];
-        __syncthreads();
+        done += (int)(total & 0xffffu);
+        met += (int)(total >> 16);
     }
-    const int m = min(done, p.keep);
+    const int m = min(done + min(met, take), p.keep);
     for (int i = m + tid; i < p.keep; i += EVICT_THREADS) kept[i] = -1;
     for (int i = m + tid; i < p.capacity; i += EVICT_THREADS) nw[i] = 0.f;
 }
