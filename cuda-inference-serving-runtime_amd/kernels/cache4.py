@@ -207,27 +207,31 @@ def tile_of(form):
 
 def launch_of(rows, segments, decode_only, heads, kv_heads, dim, dtype):
     """(form, rows of a task) for a step of `rows` rows in `segments` segments.  Forms 0 and 1: a block is 16 or 32 items whose four
-    waves share the keys; form 2: four waves of 32 items that walk the keys side by side."""
+    waves share the keys; form 2: four waves of 32 items that walk the keys side by side.
+    Microseconds by form, 0 / 1 / 2: 1,024 rows of 9 heads of 64 10 / 14 / 27, 2,048 rows 20 / 19 / 32, 8,192 rows 206 / 158 / 182; 512 rows of 32 heads of 128
+    17 / 15 / 24, 1,024 rows 33 / 34 / 46, 1,536 rows 58 / 56 / 59, 2,048 rows 92 / 81 / 77, 4,096 rows 290 / 235 / 196; 4,096 rows of 24 heads of 96
+    219 / 184 / 145; 8,192 rows of 16 heads of 64 329 / 250 / 225."""
     group = heads // kv_heads
     form = 0
     if not decode_only and dtype == torch.bfloat16 and padded(dim) <= 128:
         items = rows * group * kv_heads
-        form = 2 if items >= 128 * COMPUTE_UNITS else 1 if items >= 32 * 2 * COMPUTE_UNITS else 0
+        form = 2 if items * padded(dim) >= 96 * 256 * COMPUTE_UNITS else 1 if items >= 32 * 2 * COMPUTE_UNITS else 0
     return form, 1 if decode_only else max(1, tile_of(form) // group)
 
 
 def pieces_for(kv_heads, group, rows_per_task, form, decode_only):
-    """Pieces that all keys of a step are cut into, at least: blocks for four a compute unit, for two where rows of a prompt make many tiles anyway."""
+    """Pieces that all keys of a step are cut into, at least: blocks for four a compute unit, for two where rows of a prompt make many tiles anyway.
+    (Two, three, four, six and eight of single tokens: 32 of 16k keys 87, 86, 76, 79, 78 us, 8 of 4k keys 19, 17, 17, 18, 19.  Of prompts one, two, three:
+    64 rows behind 8,000 keys 35, 31, 31 us, 3,000 rows behind 3,000 97, 96, 96.)"""
     return max(1, (4 if decode_only else 2) * COMPUTE_UNITS // (kv_heads * -(-rows_per_task * group // tile_of(form))))
 
 
 def fill_pieces(tasks, merges, counts, cached, rows_per_task, pieces, window, turn=0):
     """Writes the tasks of a step (int32 [n, 8], see csrc/cache4_attention.inc) and its merges ([m, 4]: first row, rows, first piece, pieces; -1: none),
     unused ones at the end; returns how many tasks and merges there are.  Tiles of `rows_per_task` rows of a segment; the keys of long
-    ones are cut so that all pieces are about as long as `pieces` of them would be, the longest first; of the second `turn` tasks, which join the first
-on their compute units, the longest last.  (2,048 rows of 9 heads of 64: 21.8 us without that, 20.5 with it; 4,000 rows of 32 heads of 128: 307, 296.
-Single rows are cut from one and a half such lengths on.  Tiles of a prompt from two on, which leaves one from the first key on whole: 21.4 us and 4 for the
-merge when they are cut, 21.8 when not.)"""
+    ones are cut so that all pieces are about as long as `pieces` of them would be, the longest first; of the second `turn` tasks, which join the
+    first on their compute units, the longest last.  (2,048 rows of 9 heads of 64: 21.8 us without that, 20.5 with it; 4,000 rows of 32 heads of
+    128: 307, 296.  Where there are as many tiles as pieces anyway none is cut: 2,048 rows take 18.5 us whole, and 26 when the longer ones are cut.)"""
     counts, cached = np.asarray(counts, dtype=np.int64), np.asarray(cached, dtype=np.int64)
     tiles = -(-counts // rows_per_task)
     n = int(tiles.sum())
@@ -239,7 +243,7 @@ merge when they are cut, 21.8 when not.)"""
     first = np.maximum(0, sees - window) // STEP if window else np.zeros(n, dtype=np.int64)
     steps = -(-(sees + rows - 1) // STEP) - first
     each = max(LEAST_PIECE, -(-int(steps.sum()) // pieces))
-    cuts = np.where(steps >= (1.5 if rows_per_task == 1 else 2) * each, -(-steps // each), 1)
+    cuts = np.where((2 * steps >= 3 * each) & (n < pieces), -(-steps // each), 1)
     share = -(-steps // cuts)
     cuts = -(-steps // share)
     of = np.repeat(np.arange(n), cuts)
