@@ -160,7 +160,7 @@ def rope_write(qkv, positions, slots, cos, sin, pages, q, heads, kv_heads, dim, 
     """Turns queries and keys of the fused projection rows qkv [T, (heads + 2 kv_heads) dim] by the angles of `positions` int32 [T]
     (cos, sin float [max_pos, rot / 2]; pair i of a head is coordinates (i, i + rot / 2), or with `interleaved` (2 i, 2 i + 1)), puts
     the queries into q [T, heads dim] and holds keys and values in the token slots `slots` int32 [T] of `pages` [n, kv_heads, bytes];
-    a slot that is none (-1) is not written.  qkv stays as it is.  What is held is finite: a NaN becomes zero, an infinity the
+    a slot that is none (-1) is not written, and none may be there twice.  Positions outside the table are taken as the nearest in it.  qkv stays as it is.  What is held is finite: a NaN becomes zero, an infinity the
     largest number held."""
     record = _record(heads, kv_heads, dim, page_size)
     index = _gpu_of(qkv, "qkv", 2)
@@ -297,6 +297,7 @@ class Plan:
     heads: int
     kv_heads: int
     dim: int
+    window: int                        # of the keys that a row sees; 0: all of them
     form: int
     rows_per_task: int
     tasks: torch.Tensor                # int32 [n, 8]
@@ -365,17 +366,19 @@ def _plan(counts, cached, heads, kv_heads, dim, window, device, state_slots, for
         firsts = np.concatenate(([0], np.cumsum(counts)[:-1]))
         listed = torch.from_numpy(np.stack([firsts, counts, cached, slots], 1).astype(np.int32)).to(device)
     parts = int(tasks[:n, 6].max()) + 1
-    return Plan(rows, segments, longest, heads, kv_heads, dim, form, per_task, torch.from_numpy(tasks[:n]).to(device),
+    return Plan(rows, segments, longest, heads, kv_heads, dim, window, form, per_task, torch.from_numpy(tasks[:n]).to(device),
                 torch.from_numpy(merges[:m]).to(device) if m else None, parts, listed, 0 if listed is None else 1 + max(slots),
                 0 if listed is None else shares_of(rows, segments, longest, heads // kv_heads, kv_heads))
 
 
-def _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, what):
+def _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, window, what):
     """(GPU, bytes of a head's page, pages) of a planned step, checked against its plan."""
     record = _record(heads, kv_heads, dim, page_size)
     index = _gpu_of(q, "q", 2)
     if not isinstance(plan, Plan) or (plan.heads, plan.kv_heads, plan.dim) != (heads, kv_heads, dim):
         raise KernelError(f"{what}: the plan is of other heads")
+    if plan.window != (window or 0):
+        raise KernelError(f"{what}: a window of {window} keys, planned: {plan.window}")
     if q.dtype not in _DT or (plan.form > 0 and q.dtype is not torch.bfloat16):
         raise KernelError(f"{what}: rows in {q.dtype}: bfloat16 or float32, as planned")
     if plan.index != index or _gpu_of(pages, "pages", 3) != index:
@@ -392,7 +395,7 @@ def attention(q, pages, tables, plan, out, heads, kv_heads, dim, page_size, scal
     the block tables `tables` int32 [S, W].  Keys behind the table's end, and keys in a page that is none, are not seen; a row that sees
     none gets zeros.  `stats` float [T, heads]: gets the scores' log-sum-exp in powers of two (-inf for a row that sees none), as
     `add_weights` takes it.  Rows that the plan does not name are left as they are."""
-    index, record, n = _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, "attention")
+    index, record, n = _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, window, "attention")
     dtype, rows = q.dtype, plan.rows
     op = _t(out, "out", dtype, (rows, heads * dim), index, 8)
     sp = None if stats is None else _t(stats, "stats", torch.float32, (rows, heads), index)
@@ -403,7 +406,7 @@ def attention(q, pages, tables, plan, out, heads, kv_heads, dim, page_size, scal
     dt = _DT[dtype]
     _launch(f"cisr_attn4_d{padded(dim)}", index, _t(q, "q", dtype, (rows, heads * dim), index, 16), _t(pages, "pages", torch.uint8, (n, kv_heads, record), index, 16),
             _t(tables, "tables", torch.int32, tables.shape, index), plan.tasks.data_ptr(), op, sp, po, pm, n, plan.tasks.shape[0], plan.rows_per_task, heads,
-            kv_heads, dim, page_size, tables.shape[1], _window(window), _scale(scale), plan.form, dt)
+            kv_heads, dim, page_size, tables.shape[1], plan.window, _scale(scale), plan.form, dt)
     if plan.merges is not None:
         _launch("cisr_merge4", index, po, pm, plan.merges.data_ptr(), op, sp, plan.merges.shape[0], plan.rows_per_task, heads, kv_heads, dim, dt)
     return out
@@ -413,7 +416,7 @@ def add_weights(q, stats, pages, tables, plan, weights, heads, kv_heads, dim, pa
     """weights[slot, key head, key] += the key's attention weight, summed over the segment's rows that see it and the query heads
     that share the key head.  `stats`: what `attention` left for the same rows; weights float [slots, kv_heads, capacity], capacity at least the
     keys of the longest segment.  The same bits every time: a key's sum has one writer."""
-    index, record, n = _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, "add_weights")
+    index, record, n = _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, window, "add_weights")
     if plan.segments is None:
         raise KernelError("add_weights: the plan names no state slots")
     if _gpu_of(weights, "weights", 3) != index or weights.shape[1] != kv_heads or weights.shape[2] < plan.span or weights.shape[0] < plan.slots_below:
@@ -425,7 +428,7 @@ def add_weights(q, stats, pages, tables, plan, weights, heads, kv_heads, dim, pa
     _launch(f"cisr_weights4_d{padded(dim)}", index, _t(q, "q", q.dtype, (plan.rows, heads * dim), index, 16),
             _t(stats, "stats", torch.float32, (plan.rows, heads), index), _t(pages, "pages", torch.uint8, (n, kv_heads, record), index, 16),
             _t(tables, "tables", torch.int32, tables.shape, index), plan.segments.data_ptr(), _t(weights, "weights", torch.float32, weights.shape, index),
-            None if plan.shares < 2 else plan.room.data_ptr(), n, plan.n_segments, plan.span, heads, kv_heads, dim, page_size, tables.shape[1], _window(window),
+            None if plan.shares < 2 else plan.room.data_ptr(), n, plan.n_segments, plan.span, heads, kv_heads, dim, page_size, tables.shape[1], plan.window,
             capacity, slots, _scale(scale), plan.shares, blocks, _DT[q.dtype])
     return weights
 
@@ -437,7 +440,8 @@ def evict(storage, weights, tables, new_tables, lengths, slots, new_slots, kv_he
     of attention weight, `keep` in all (all of them where there are no more); of equal sums the earlier key stays, a NaN counts least.
     The kept keys and values go, in their order, from the pages of `tables` int32 [R, W] to those of `new_tables` int32 [R, W'] (other
     pages, W' page_size at least `keep`) at every site of `storage` [sites, n, kv_heads, bytes]; their sums from weights[site][slots[r]]
-    to weights[site][new_slots[r]] (float [n_slots, kv_heads, capacity] a site; it may be the same slot), zeros behind them.
+    to weights[site][new_slots[r]] (float [n_slots, kv_heads, capacity] a site; it may be the request's own old slot, never another request's, old or new),
+    zeros behind them.  Of a request without keys nothing is read or written but its -1 in `kept`.
     kept int32 [sites, R, kv_heads, keep] gets their indices, -1 behind the last.  lengths, slots, new_slots: int32 [R]."""
     record = _record(kv_heads, kv_heads, dim, page_size)
     keep, recent = operator.index(keep), operator.index(recent)
@@ -572,7 +576,7 @@ def attend(ctx, q, pages, view, out, heads, kv_heads, dim, scale, window=None, s
         shares = shares_of(rows, S, span, heads // kv_heads, kv_heads)
     pieces = n_tasks if split else 0
     floats = max(pieces * per_task * heads * (dim + 2), shares * S * kv_heads * span if shares > 1 else 0)
-    plan = Plan(rows, S, span, heads, kv_heads, dim, form, per_task, words[:8 * min(n_tasks, most)].view(-1, 8), words[len(words) - 4 * merges:].view(-1, 4) if split else None,
+    plan = Plan(rows, S, span, heads, kv_heads, dim, _window(window), form, per_task, words[:8 * min(n_tasks, most)].view(-1, 8), words[len(words) - 4 * merges:].view(-1, 4) if split else None,
                 pieces, segments, 0 if sums is None else sums.shape[0], shares, ctx.buffer("cache4.room", (floats,), torch.float32) if floats else None)
     stats = None if sums is None else ctx.buffer("cache4.stats", (rows, heads), torch.float32)
     attention(q, pages, view.tables, plan, out, heads, kv_heads, dim, view.page_size, scale, window, stats)
