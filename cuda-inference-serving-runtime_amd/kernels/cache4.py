@@ -119,9 +119,12 @@ def _gpu_of(t, name, dims):
     return t.get_device()
 
 
-def _pool(pages, what):
-    """How many pages a pool has (page numbers are 32-bit)."""
-    n = pages.shape[-3]
+def _pool(pages, name, dims, what):
+    """How many pages a pool of so many dimensions has (page numbers are 32-bit)."""
+    shape = pages.shape if isinstance(pages, torch.Tensor) else ()
+    if len(shape) != dims:
+        raise KernelError(f"{name}: expected a GPU tensor of {dims} dimensions")
+    n = shape[-3]
     if not 0 < n < 1 << 31:
         raise KernelError(f"{what}: a pool of {n} pages")
     return n
@@ -137,6 +140,11 @@ def _launch(name, index, *args):
             code = fn(*args, ops._stream())
     if code:
         raise KernelError(f"{name}: HIP error {code}")
+
+
+@functools.lru_cache(maxsize=256)
+def _of_size(name, dim):
+    return f"{name}{padded(dim)}"
 
 
 def _scale(scale):
@@ -167,11 +175,9 @@ def rope_write(qkv, positions, slots, cos, sin, pages, q, heads, kv_heads, dim, 
     dtype, rows = qkv.dtype, qkv.shape[0]
     if dtype not in _DT:
         raise KernelError("qkv: expected rows of bfloat16 or float32")
-    if cos.dim() != 2 or not 0 < 2 * cos.shape[1] <= dim or cos.shape[0] == 0:
-        raise KernelError(f"rope_write: angles {tuple(cos.shape)} do not fit heads of {dim}")
-    if _gpu_of(pages, "pages", 3) != index:
-        raise KernelError("rope_write: pages and rows on different GPUs")
-    n, table = _pool(pages, "rope_write"), cos.shape
+    n, table = _pool(pages, "pages", 3, "rope_write"), cos.shape
+    if len(table) != 2 or not 0 < 2 * table[1] <= dim or table[0] == 0:
+        raise KernelError(f"rope_write: angles {tuple(table)} do not fit heads of {dim}")
     if rows:
         _launch("cisr_write4", index, _t(qkv, "qkv", dtype, (rows, (heads + 2 * kv_heads) * dim), index), _t(positions, "positions", torch.int32, (rows,), index),
                 _t(slots, "slots", torch.int32, (rows,), index), _t(cos, "cos", torch.float32, table, index), _t(sin, "sin", torch.float32, table, index),
@@ -185,7 +191,7 @@ def read(storage, slots, keys, values, kv_heads, dim, page_size):
     [sites, T, kv_heads, dim], exactly; zeros for a slot that is none."""
     record = _record(kv_heads, kv_heads, dim, page_size)
     index = _gpu_of(storage, "storage", 4)
-    n, sites, rows = _pool(storage, "read"), storage.shape[0], slots.shape[0]
+    n, sites, rows = _pool(storage, "storage", 4, "read"), storage.shape[0], slots.shape[0]
     shape = (sites, rows, kv_heads, dim)
     if rows and sites:
         _launch("cisr_read4", index, _t(storage, "storage", torch.uint8, (sites, n, kv_heads, record), index, 16), _t(slots, "slots", torch.int32, (rows,), index),
@@ -372,7 +378,7 @@ def _plan(counts, cached, heads, kv_heads, dim, window, device, state_slots, for
 
 
 def _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, window, what):
-    """(GPU, bytes of a head's page, pages) of a planned step, checked against its plan."""
+    """(GPU, bytes of a head's page, pages, the tables' shape) of a planned step, checked against its plan."""
     record = _record(heads, kv_heads, dim, page_size)
     index = _gpu_of(q, "q", 2)
     if not isinstance(plan, Plan) or (plan.heads, plan.kv_heads, plan.dim) != (heads, kv_heads, dim):
@@ -381,11 +387,12 @@ def _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, window, wh
         raise KernelError(f"{what}: a window of {window} keys, planned: {plan.window}")
     if q.dtype not in _DT or (plan.form > 0 and q.dtype is not torch.bfloat16):
         raise KernelError(f"{what}: rows in {q.dtype}: bfloat16 or float32, as planned")
-    if plan.index != index or _gpu_of(pages, "pages", 3) != index:
-        raise KernelError(f"{what}: rows, pages and plan on different GPUs")
-    if tables.dim() != 2 or tables.shape[0] < plan.n_segments or not 0 < tables.shape[1] * page_size < 1 << 31:
-        raise KernelError(f"tables: shape {tuple(tables.shape)} for {plan.n_segments} segments")
-    return index, record, _pool(pages, what)
+    if plan.index != index:
+        raise KernelError(f"{what}: rows and plan on different GPUs")
+    shape = tables.shape
+    if len(shape) != 2 or shape[0] < plan.n_segments or not 0 < shape[1] * page_size < 1 << 31:
+        raise KernelError(f"tables: shape {tuple(shape)} for {plan.n_segments} segments")
+    return index, record, _pool(pages, "pages", 3, what), shape
 
 
 # -- attention ------------------------------------------------------------------------------------------------------
@@ -395,7 +402,7 @@ def attention(q, pages, tables, plan, out, heads, kv_heads, dim, page_size, scal
     the block tables `tables` int32 [S, W].  Keys behind the table's end, and keys in a page that is none, are not seen; a row that sees
     none gets zeros.  `stats` float [T, heads]: gets the scores' log-sum-exp in powers of two (-inf for a row that sees none), as
     `add_weights` takes it.  Rows that the plan does not name are left as they are."""
-    index, record, n = _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, window, "attention")
+    index, record, n, table = _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, window, "attention")
     dtype, rows = q.dtype, plan.rows
     op = _t(out, "out", dtype, (rows, heads * dim), index, 8)
     sp = None if stats is None else _t(stats, "stats", torch.float32, (rows, heads), index)
@@ -404,9 +411,9 @@ def attention(q, pages, tables, plan, out, heads, kv_heads, dim, page_size, scal
         po = plan.room.data_ptr()
         pm = po + 4 * plan.pieces * plan.rows_per_task * heads * dim
     dt = _DT[dtype]
-    _launch(f"cisr_attn4_d{padded(dim)}", index, _t(q, "q", dtype, (rows, heads * dim), index, 16), _t(pages, "pages", torch.uint8, (n, kv_heads, record), index, 16),
-            _t(tables, "tables", torch.int32, tables.shape, index), plan.tasks.data_ptr(), op, sp, po, pm, n, plan.tasks.shape[0], plan.rows_per_task, heads,
-            kv_heads, dim, page_size, tables.shape[1], plan.window, _scale(scale), plan.form, dt)
+    _launch(_of_size("cisr_attn4_d", dim), index, _t(q, "q", dtype, (rows, heads * dim), index, 16), _t(pages, "pages", torch.uint8, (n, kv_heads, record), index, 16),
+            _t(tables, "tables", torch.int32, table, index), plan.tasks.data_ptr(), op, sp, po, pm, n, plan.tasks.shape[0], plan.rows_per_task, heads,
+            kv_heads, dim, page_size, table[1], plan.window, _scale(scale), plan.form, dt)
     if plan.merges is not None:
         _launch("cisr_merge4", index, po, pm, plan.merges.data_ptr(), op, sp, plan.merges.shape[0], plan.rows_per_task, heads, kv_heads, dim, dt)
     return out
@@ -416,7 +423,7 @@ def add_weights(q, stats, pages, tables, plan, weights, heads, kv_heads, dim, pa
     """weights[slot, key head, key] += the key's attention weight, summed over the segment's rows that see it and the query heads
     that share the key head.  `stats`: what `attention` left for the same rows; weights float [slots, kv_heads, capacity], capacity at least the
     keys of the longest segment.  The same bits every time: a key's sum has one writer."""
-    index, record, n = _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, window, "add_weights")
+    index, record, n, table = _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, window, "add_weights")
     if plan.segments is None:
         raise KernelError("add_weights: the plan names no state slots")
     if _gpu_of(weights, "weights", 3) != index or weights.shape[1] != kv_heads or weights.shape[2] < plan.span or weights.shape[0] < plan.slots_below:
@@ -425,10 +432,10 @@ def add_weights(q, stats, pages, tables, plan, weights, heads, kv_heads, dim, pa
     # 16 rows of 2k keys, 8 key heads: 4, 6, 8, 12 and 17 blocks each (6 is the rule's) take 10.4, 8.7, 11.3, 10.7 and 10.9 us.
     blocks = max(1, min(-(-plan.span // (4 * STEP)), -(-3 * COMPUTE_UNITS // (kv_heads * plan.n_segments))))
     slots, _, capacity = weights.shape
-    _launch(f"cisr_weights4_d{padded(dim)}", index, _t(q, "q", q.dtype, (plan.rows, heads * dim), index, 16),
+    _launch(_of_size("cisr_weights4_d", dim), index, _t(q, "q", q.dtype, (plan.rows, heads * dim), index, 16),
             _t(stats, "stats", torch.float32, (plan.rows, heads), index), _t(pages, "pages", torch.uint8, (n, kv_heads, record), index, 16),
-            _t(tables, "tables", torch.int32, tables.shape, index), plan.segments.data_ptr(), _t(weights, "weights", torch.float32, weights.shape, index),
-            None if plan.shares < 2 else plan.room.data_ptr(), n, plan.n_segments, plan.span, heads, kv_heads, dim, page_size, tables.shape[1], plan.window,
+            _t(tables, "tables", torch.int32, table, index), plan.segments.data_ptr(), _t(weights, "weights", torch.float32, weights.shape, index),
+            None if plan.shares < 2 else plan.room.data_ptr(), n, plan.n_segments, plan.span, heads, kv_heads, dim, page_size, table[1], plan.window,
             capacity, slots, _scale(scale), plan.shares, blocks, _DT[q.dtype])
     return weights
 
@@ -448,7 +455,7 @@ def evict(storage, weights, tables, new_tables, lengths, slots, new_slots, kv_he
     if not 0 < keep < 1 << 30 or not 0 <= recent <= keep:
         raise KernelError(f"evict: {recent} last keys of {keep}")
     index = _gpu_of(storage, "storage", 4)
-    n, sites, requests = _pool(storage, "evict"), storage.shape[0], lengths.shape[0]
+    n, sites, requests = _pool(storage, "storage", 4, "evict"), storage.shape[0], lengths.shape[0]
     if len(weights) != sites or sites == 0:
         raise KernelError(f"evict: sums of {len(weights)} sites for {sites}")
     _gpu_of(weights[0], "weights", 3)
