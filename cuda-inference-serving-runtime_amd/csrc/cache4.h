@@ -27,3 +27,17 @@ __device__ __forceinline__ int cache4_value_at(int dp, int shift, int t, int d) 
 __device__ __forceinline__ int cache4_scale_at(int dp, int shift, int t, int block, bool value) {
     return (dp << shift) + (((value ? dp / 32 : 0) + block) << shift) + t;
 }
+
+// Calls of the entry points that there is one of for each head size.
+struct Attn4Call {
+    hipStream_t stream; const void* q; const uint8_t* pages; const int* tables; const int* tasks; void* out; float* stats; float* part_o; float* part_ml;
+    long long n_pages;
+    int n_tasks, rows_per_task, heads, kv_heads, dim, page, width, window, form, dtype;
+    float scale;
+};
+struct Weights4Call {
+    hipStream_t stream; const void* q; const float* stats; const uint8_t* pages; const int* tables; const int* segments; float* weights; float* parts;
+    long long n_pages;
+    int n_segments, span, heads, kv_heads, dim, page, width, window, capacity, n_slots, shares, blocks, dtype;
+    float scale;
+};

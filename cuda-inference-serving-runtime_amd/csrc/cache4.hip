@@ -529,10 +529,28 @@ merge4_kernel(Merge4Args p) {
     if (p.stats && d == 0) p.stats[to] = m + log2f(l);
 }
 
+// What an entry point is called with, one block of bytes (a pointer to it is converted in a tenth of the time of 20 arguments, 1 us of 9 a call).
+struct Write4Call {
+    hipStream_t stream; const void* qkv; const int* positions; const int* slots; const float* cos; const float* sin; uint8_t* pages; void* q;
+    int rows, heads, kv_heads, dim, rot, page, n_pages, max_pos, interleaved, dtype;
+};
+struct Read4Call { hipStream_t stream; const uint8_t* pages; const int* slots; bf16_t* keys; bf16_t* values; int sites, rows, kv_heads, dim, page, n_pages; };
+struct Evict4Call {
+    hipStream_t stream; const int* lengths; const int* slots; const int* new_slots; const int* tables; const int* new_tables; uint8_t* pages; int* kept;
+    int sites, n_pages, requests, kv_heads, dim, page, width, new_width, keep, recent, capacity, n_slots;
+};
+struct Merge4Call { hipStream_t stream; const float* part_o; const float* part_ml; const int* merges; void* out; float* stats; int n, rows_per_task, heads, kv_heads, dim, dtype; };
+
 extern "C" {
 
-int cisr_write4(const void* qkv, const int* positions, const int* slots, const float* cos, const float* sin, void* pages, void* q, int rows, int heads,
-                int kv_heads, int dim, int rot, int page, int n_pages, int max_pos, int interleaved, int dtype, void* stream) {
+// Bytes of a call as it is here, by entry point: what the caller packs has to agree.
+int cisr_call4_bytes(int which) {
+    const size_t bytes[] = {sizeof(Write4Call), sizeof(Read4Call), sizeof(Evict4Call), sizeof(Merge4Call), sizeof(Attn4Call), sizeof(Weights4Call)};
+    return which >= 0 && which < 6 ? (int)bytes[which] : -1;
+}
+
+int cisr_write4(const Write4Call* call) {
+    const auto [stream, qkv, positions, slots, cos, sin, pages, q, rows, heads, kv_heads, dim, rot, page, n_pages, max_pos, interleaved, dtype] = *call;
     if (rows <= 0 || heads <= 0 || kv_heads <= 0 || dim <= 0 || dim > 256 || dim % 2 || rot < 0 || rot > dim || rot % 2 || page < 8 || (page & (page - 1)) || n_pages <= 0 || max_pos <= 0)
         return hipErrorInvalidValue;
     const int dp = (dim + 31) / 32 * 32;
@@ -555,7 +573,8 @@ int cisr_write4(const void* qkv, const int* positions, const int* slots, const f
     return hipGetLastError();
 }
 
-int cisr_read4(const void* pages, const int* slots, void* keys, void* values, int sites, int rows, int kv_heads, int dim, int page, int n_pages, void* stream) {
+int cisr_read4(const Read4Call* call) {
+    const auto [stream, pages, slots, keys, values, sites, rows, kv_heads, dim, page, n_pages] = *call;
     if (sites <= 0 || rows <= 0 || kv_heads <= 0 || dim <= 0 || dim > 256 || dim % 2 || page < 8 || (page & (page - 1)) || n_pages <= 0) return hipErrorInvalidValue;
     const long long pieces = (long long)rows * kv_heads * 2 * ((dim + 7) / 8);
     if (pieces > INT32_MAX || sites > 65535) return hipErrorInvalidValue;
@@ -564,8 +583,9 @@ int cisr_read4(const void* pages, const int* slots, void* keys, void* values, in
     return hipGetLastError();
 }
 
-int cisr_evict4(const int* lengths, const int* slots, const int* new_slots, const int* tables, const int* new_tables, void* pages, void* const* weights, int* kept,
-                int sites, int n_pages, int requests, int kv_heads, int dim, int page, int width, int new_width, int keep, int recent, int capacity, int n_slots, void* stream) {
+int cisr_evict4(const Evict4Call* call, void* const* weights) {
+    const auto [stream, lengths, slots, new_slots, tables, new_tables, pages, kept, sites, n_pages, requests, kv_heads, dim, page, width, new_width, keep, recent, capacity,
+                n_slots] = *call;
     if (sites <= 0 || n_pages <= 0 || requests <= 0 || requests > 65535 || kv_heads <= 0 || dim <= 0 || dim > 256 || page < 8 || (page & (page - 1)) || width <= 0 || new_width <= 0 || keep <= 0 ||
         recent < 0 || recent > keep || capacity < keep || n_slots <= 0)
         return hipErrorInvalidValue;
@@ -588,8 +608,8 @@ int cisr_evict4(const int* lengths, const int* slots, const int* new_slots, cons
     return hipSuccess;
 }
 
-int cisr_merge4(const float* part_o, const float* part_ml, const int* merges, void* out, float* stats, int n, int rows_per_task, int heads, int kv_heads, int dim, int dtype,
-                void* stream) {
+int cisr_merge4(const Merge4Call* call) {
+    const auto [stream, part_o, part_ml, merges, out, stats, n, rows_per_task, heads, kv_heads, dim, dtype] = *call;
     if (n <= 0 || rows_per_task <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dim <= 0 || dim % 2) return hipErrorInvalidValue;
     const long long blocks = ((long long)rows_per_task * heads * (dim / 2) + 255) / 256;
     if (blocks > 65535) return hipErrorInvalidValue;

@@ -20,6 +20,7 @@ import ctypes as C
 import functools
 import math
 import operator
+import struct
 from dataclasses import dataclass
 from typing import Optional
 
@@ -49,23 +50,23 @@ def supported(dim, page_size):
     return 0 < dim <= MAX_HEAD and dim % 2 == 0 and page_size >= 8 and page_size & (page_size - 1) == 0
 
 
+# What an entry point takes: a block of bytes with the stream first, laid out as csrc/cache4.hip and cache4.h say (`cisr_call4_bytes` knows them by
+# their place here).  ctypes converts 20 arguments in 1.3 us, a pointer to 20 that are packed in 0.4.
+_CALLS = {"cisr_write4": "8P10i", "cisr_read4": "5P6i", "cisr_evict4": "8P12i", "cisr_merge4": "6P6i", "cisr_attn4": "9Pq10if", "cisr_weights4": "8Pq13if"}
+
+
 def _entry(name):
-    fn = _entries.get(name)
-    if fn is None:
-        p, i, f, ll = C.c_void_p, C.c_int, C.c_float, C.c_longlong
-        kind = name.split("_d")[0]
-        fn = getattr(library.load(UNIT), name)
-        fn.argtypes = {
-            "cisr_write4": [p, p, p, p, p, p, p, i, i, i, i, i, i, i, i, i, i, p],
-            "cisr_read4": [p, p, p, p, i, i, i, i, i, i, p],
-            "cisr_evict4": [p, p, p, p, p, p, p, p, i, i, i, i, i, i, i, i, i, i, i, i, p],
-            "cisr_merge4": [p, p, p, p, p, i, i, i, i, i, i, p],
-            "cisr_attn4": [p, p, p, p, p, p, p, p, ll, i, i, i, i, i, i, i, i, f, i, i, p],
-            "cisr_weights4": [p, p, p, p, p, p, p, ll, i, i, i, i, i, i, i, i, i, i, f, i, i, i, p],
-        }[kind]
+    found = _entries.get(name)
+    if found is None:
+        lib, kind = library.load(UNIT), name.split("_d")[0]
+        call = struct.Struct(_CALLS[kind] + "0P")                  # (filled up to whole pointers, as the compiler does)
+        if lib.cisr_call4_bytes(list(_CALLS).index(kind)) != call.size:
+            raise library.KernelLibraryError(f"{name}: its arguments take {call.size} bytes here and others in the library")
+        fn = getattr(lib, name)
+        fn.argtypes = [C.c_char_p, C.c_char_p][:2 if kind == "cisr_evict4" else 1]
         fn.restype = C.c_int
-        _entries[name] = fn
-    return fn
+        found = _entries[name] = (fn, call.pack)
+    return found
 
 
 def _t(t, name, dtype, shape, index, align=1):
@@ -130,14 +131,17 @@ def _pool(pages, name, dims, what):
     return n
 
 
-def _launch(name, index, *args):
+def _launch(name, index, *args, more=()):
     """Runs an entry point on the current stream of GPU `index`."""
-    fn = _entries.get(name) or _entry(name)
-    if ops._raw_stream is not None and ops._current_device is not None and ops._current_device() == index:
-        code = fn(*args, ops._raw_stream(index))
-    else:
-        with torch.cuda.device(index):
-            code = fn(*args, ops._stream())
+    fn, pack = _entries.get(name) or _entry(name)
+    try:
+        if ops._raw_stream is not None and ops._current_device is not None and ops._current_device() == index:
+            code = fn(pack(ops._raw_stream(index), *args), *more)
+        else:
+            with torch.cuda.device(index):
+                code = fn(pack(ops._stream(), *args), *more)
+    except struct.error as e:
+        raise KernelError(f"{name}: {e}") from None
     if code:
         raise KernelError(f"{name}: HIP error {code}")
 
@@ -405,15 +409,15 @@ def attention(q, pages, tables, plan, out, heads, kv_heads, dim, page_size, scal
     index, record, n, table = _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, window, "attention")
     dtype, rows = q.dtype, plan.rows
     op = _t(out, "out", dtype, (rows, heads * dim), index, 8)
-    sp = None if stats is None else _t(stats, "stats", torch.float32, (rows, heads), index)
-    po = pm = None
+    sp = 0 if stats is None else _t(stats, "stats", torch.float32, (rows, heads), index)
+    po = pm = 0
     if plan.pieces:
         po = plan.room.data_ptr()
         pm = po + 4 * plan.pieces * plan.rows_per_task * heads * dim
     dt = _DT[dtype]
     _launch(_of_size("cisr_attn4_d", dim), index, _t(q, "q", dtype, (rows, heads * dim), index, 16), _t(pages, "pages", torch.uint8, (n, kv_heads, record), index, 16),
             _t(tables, "tables", torch.int32, table, index), plan.tasks.data_ptr(), op, sp, po, pm, n, plan.tasks.shape[0], plan.rows_per_task, heads,
-            kv_heads, dim, page_size, table[1], plan.window, _scale(scale), plan.form, dt)
+            kv_heads, dim, page_size, table[1], plan.window, plan.form, dt, _scale(scale))
     if plan.merges is not None:
         _launch("cisr_merge4", index, po, pm, plan.merges.data_ptr(), op, sp, plan.merges.shape[0], plan.rows_per_task, heads, kv_heads, dim, dt)
     return out
@@ -435,8 +439,8 @@ def add_weights(q, stats, pages, tables, plan, weights, heads, kv_heads, dim, pa
     _launch(_of_size("cisr_weights4_d", dim), index, _t(q, "q", q.dtype, (plan.rows, heads * dim), index, 16),
             _t(stats, "stats", torch.float32, (plan.rows, heads), index), _t(pages, "pages", torch.uint8, (n, kv_heads, record), index, 16),
             _t(tables, "tables", torch.int32, table, index), plan.segments.data_ptr(), _t(weights, "weights", torch.float32, weights.shape, index),
-            None if plan.shares < 2 else plan.room.data_ptr(), n, plan.n_segments, plan.span, heads, kv_heads, dim, page_size, table[1], plan.window,
-            capacity, slots, _scale(scale), plan.shares, blocks, _DT[q.dtype])
+            0 if plan.shares < 2 else plan.room.data_ptr(), n, plan.n_segments, plan.span, heads, kv_heads, dim, page_size, table[1], plan.window,
+            capacity, slots, plan.shares, blocks, _DT[q.dtype], _scale(scale))
     return weights
 
 
@@ -469,9 +473,9 @@ def evict(storage, weights, tables, new_tables, lengths, slots, new_slots, kv_he
         _launch("cisr_evict4", index, _t(lengths, "lengths", torch.int32, (requests,), index), _t(slots, "slots", torch.int32, (requests,), index),
                 _t(new_slots, "new_slots", torch.int32, (requests,), index), _t(tables, "tables", torch.int32, (requests, tables.shape[1]), index),
                 _t(new_tables, "new_tables", torch.int32, (requests, new_tables.shape[1]), index),
-                _t(storage, "storage", torch.uint8, (sites, n, kv_heads, record), index, 16), (C.c_void_p * sites)(*sums),
+                _t(storage, "storage", torch.uint8, (sites, n, kv_heads, record), index, 16),
                 _t(kept, "kept", torch.int32, (sites, requests, kv_heads, keep), index), sites, n, requests, kv_heads, dim, page_size, tables.shape[1],
-                new_tables.shape[1], keep, recent, capacity, n_slots)
+                new_tables.shape[1], keep, recent, capacity, n_slots, more=(struct.pack(f"{sites}P", *sums),))
     return kept
 
 
