@@ -207,9 +207,13 @@ class ModelRunner:
             raise
         self.cache.commit(done)
         if getattr(self.model, "kept_keys", None):
-            for d in done:
-                if self.cache.overfull(d.request):
-                    self._give_up(d.request)
+            try:
+                for d in done:
+                    if self.cache.overfull(d.request):
+                        self._give_up(d.request)
+            except BaseException:
+                self._failed.update(e.request for e in entries)      # (pages that hold nothing yet, and logits that nobody got)
+                raise
         self.steps += 1
         self.counters["steps"] += 1
         if logits is None:

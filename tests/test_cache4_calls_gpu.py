@@ -384,3 +384,28 @@ def test_calls_that_are_refused():
     with pytest.raises(KernelError):
         c.attention(s.q, s.storage[0], s.tables, s.plan, s.out, 6, 2, 64, 16, 0.125, stats=s.stats[:, :5])
     same(run.got(), before)
+
+
+def test_a_request_whose_keys_could_not_be_moved_is_only_released(folders, monkeypatch):
+    from conftest import TINY, random_tokens
+    from test_cache4_engine_gpu import make_runner
+    from runtime.engine.runner import StepEntry
+    from runtime.kernels.ops import KernelError
+    runner = make_runner(folders["a"], "float32", keep=16, recent=4, slack=8, portion=16)
+    tokens = random_tokens(4, 40, TINY["a"]["vocab_size"])
+
+    def fails(*args):
+        raise KernelError("no")
+    runner.create("x")
+    runner.step([StepEntry("x", tokens[:16], [])])
+    with monkeypatch.context() as m:
+        m.setattr(cache4(), "evict", fails)
+        with pytest.raises(KernelError):
+            runner.step([StepEntry("x", tokens[16:32], [15])])
+    with pytest.raises(Exception, match="x"):
+        runner.step([StepEntry("x", tokens[32:33], [0])])
+    runner.cache.check()
+    runner.release("x")
+    runner.create("x")
+    runner.step([StepEntry("x", tokens[:16], [])])
+    assert runner.step([StepEntry("x", tokens[16:32], [15])]).isfinite().all() and runner.cache.cached("x") == 16
