@@ -409,3 +409,35 @@ def test_a_request_whose_keys_could_not_be_moved_is_only_released(folders, monke
     runner.create("x")
     runner.step([StepEntry("x", tokens[:16], [])])
     assert runner.step([StepEntry("x", tokens[16:32], [15])]).isfinite().all() and runner.cache.cached("x") == 16
+
+
+@pytest.mark.parametrize("execution", ["eager", "graph"])
+def test_a_layer_that_reads_another_layers_keys_in_4_bits(execution):
+    """Logits of a portion and of single tokens behind it against 64 bits over what the two caches hold."""
+    import numpy as np
+    import plain_llama as P
+    from conftest import assert_close
+    from test_cache4_engine_gpu import held
+    from test_norm_hand_over_gpu import EPS, THETA, model_of
+    from runtime.engine import ModelRunner, StepEntry
+    heads, kv, order = 4, 2, [(0, None), (1, 0), (0, None), (2, None)]
+    model, w, _ = model_of(128, heads, kv, 256, [{}, {"own_kv": False}, {}], order)
+    model.bind({name: torch.from_numpy(t).float().to(GPU) for name, t in w.items()}, torch.float32, torch.device(GPU))
+    model.hold_cache(4)
+    runner = ModelRunner(model, n_pages=8, page_size=16, max_requests=1, execution=execution)
+    tokens = np.random.default_rng(3).integers(0, 96, size=45)
+    runner.create("x")
+    got = [runner.step([StepEntry("x", list(tokens[:40]), list(range(40)))]).cpu().numpy()]
+    got += [runner.step([StepEntry("x", [int(t)], [0])]).cpu().numpy() for t in tokens[40:]]
+    sites = [site for site in range(len(order)) if site in runner.cache.group_of_site]
+    caches = {site: held(runner, "x", site, 45) for site in sites}
+    assert len(sites) == 3
+    x, pos = w["embed.weight"][tokens], np.arange(45)
+    for site, (layer, reads) in enumerate(order):
+        n = f"l{layer}"
+        q = P.rope(P.linear(P.rmsnorm(x, w[n + ".n1.weight"], EPS), w[n + ".attn.q_proj.weight"]).reshape(45, heads, 64), pos, THETA)
+        k, v = caches[site if reads is None else reads]
+        x = x + P.linear(P.causal_attention(q, k, v).reshape(45, heads * 64), w[n + ".attn.o_proj.weight"])
+        h = P.rmsnorm(x, w[n + ".n2.weight"], EPS)
+        x = x + P.linear(P.swiglu(P.linear(h, w[n + ".mlp.gate_proj.weight"]), P.linear(h, w[n + ".mlp.up_proj.weight"])), w[n + ".mlp.down_proj.weight"])
+    assert_close(np.concatenate(got), P.linear(P.rmsnorm(x, w["final.weight"], EPS), w["head.weight"]), "float32", execution)
