@@ -53,6 +53,39 @@ def _bucket(n):
     return 1 << (n - 1).bit_length() if n <= 64 else -(-n // 64) * 64
 
 
+class Staging:
+    """Pinned host buffers of int32 in turn, each with one on the device: what was uploaded is there until three more uploads have been made."""
+
+    def __init__(self, device):
+        self.device, self.entries, self.next, self.current = device, [None] * 4, 0, None
+
+    def stage(self, n):
+        """A pinned host buffer of at least n int32, not in flight."""
+        slot = self.next % 4
+        self.next += 1
+        entry = self.entries[slot]
+        if entry is None or entry[0].numel() < n:
+            cap = max(4096, 1 << (n - 1).bit_length())
+            entry = [torch.empty(cap, dtype=torch.int32, pin_memory=True),
+                     torch.empty(cap, dtype=torch.int32, device=self.device), None]
+            self.entries[slot] = entry
+        if entry[2] is not None:
+            entry[2].synchronize()  # the copy that last read this buffer is over
+        self.current = entry
+        return entry[0]
+
+    def upload(self, host, n, device_buffer=None):
+        entry = self.current
+        target = entry[1] if device_buffer is None else device_buffer
+        target[:n].copy_(host[:n], non_blocking=True)
+        entry[2] = torch.cuda.Event()
+        entry[2].record()
+        return target
+
+    def bytes(self):
+        return sum(4 * entry[0].numel() for entry in self.entries if entry is not None)
+
+
 class ModelRunner:
     def __init__(self, model, n_pages, page_size=16, max_requests=64, device="cuda:0", execution="eager", program_capacity=64):
         if not torch.cuda.is_available():
@@ -94,8 +127,9 @@ class ModelRunner:
         self.scratch = ops.ScratchPool(ring=not getattr(model, "routes", False))   # what products need beyond their operands (never shared with another runner)
         self.max_context = model.max_positions
         self.table_width = -(-self.max_context // page_size)
-        self._staging = []
-        self._staging_next = 0
+        # buffers of the steps' metadata, and of what moves kept keys between steps: a step's metadata has to outlive the moves behind it, as its
+        # logits' slots are read when tokens are picked
+        self._staging, self._moves = Staging(self.device), Staging(self.device)
         self._layouts = {}
         # host copies of the block tables by state slot, with the stamp of the table they were made from
         self._table_mirror = [(np.full((max_requests, self.table_width), -1, dtype=np.int32), [None] * max_requests)
@@ -231,9 +265,9 @@ class ModelRunner:
             return
         for group, (old, new) in zip(cache.groups, tables):
             n, m = len(old), len(new)
-            host = self._stage(3 + n + m)
+            host = self._moves.stage(3 + n + m)
             host[:3 + n + m] = torch.tensor([held, slot, slot, *old, *new], dtype=torch.int32)
-            dev = self._upload(host, 3 + n + m)
+            dev = self._moves.upload(host, 3 + n + m)
             need = group.need
             kept = self.workspace.get("cache4.kept", (len(group.sites), 1, need.kv_heads, keep), torch.int32)
             cache4.evict(group.storage, [cache.state_storage[site] for site in group.sites], dev[3:3 + n][None], dev[3 + n:3 + n + m][None], dev[:1], dev[1:2], dev[2:3],
@@ -324,7 +358,7 @@ class ModelRunner:
         if offsets is None:
             offsets = self._layouts[layout] = [int(x) for x in self._layout(T, S, R, W, carried)]
         total = offsets[-1]
-        host = self._stage(total)
+        host = self._staging.stage(total)
         arr = host.numpy()
         tokens, positions, seg_of_row, seg_start, seg_first, state_slots, logit_rows, token_source, logit_slots = (
             arr[offsets[i]:offsets[i + 1]] for i in range(F))
@@ -384,7 +418,7 @@ class ModelRunner:
             batch.launch_values[array] = own if launch_values is None or own is None else launch_values.get(array, 0)
         for i, array in enumerate(carried):
             array.fill(arr[offsets[F + 2 * G + i]:offsets[F + 1 + 2 * G + i]], batch, batch.launch_values[array])
-        dev = self._upload(host, total, device_buffer)
+        dev = self._staging.upload(host, total, device_buffer)
 
         def view(i, shape=None):
             t = dev[offsets[i]:offsets[i + 1]]
@@ -403,31 +437,6 @@ class ModelRunner:
         ctx.max_context = ctx.span_hint = longest
         ctx.decode_only = decode_only
         return ctx
-
-    def _stage(self, n):
-        """A pinned host buffer of at least n int32, not in flight."""
-        slot = self._staging_next % 4
-        self._staging_next += 1
-        while len(self._staging) <= slot:
-            self._staging.append(None)
-        entry = self._staging[slot]
-        if entry is None or entry[0].numel() < n:
-            cap = max(4096, 1 << (n - 1).bit_length())
-            entry = [torch.empty(cap, dtype=torch.int32, pin_memory=True),
-                     torch.empty(cap, dtype=torch.int32, device=self.device), None]
-            self._staging[slot] = entry
-        if entry[2] is not None:
-            entry[2].synchronize()  # the copy that last read this buffer is over
-        self._current = entry
-        return entry[0]
-
-    def _upload(self, host, n, device_buffer=None):
-        entry = self._current
-        target = entry[1] if device_buffer is None else device_buffer
-        target[:n].copy_(host[:n], non_blocking=True)
-        entry[2] = torch.cuda.Event()
-        entry[2].record()
-        return target
 
     # -- captured programs ------------------------------------------------------------
     def _program_key(self, entries, done):
@@ -505,7 +514,7 @@ class ModelRunner:
         steps run, how many kernel by kernel, programs captured, replayed and evicted, metadata layouts made;
         bytes of the intermediate buffers, of the products' scratch memory, of the pinned and device staging of the
         metadata, of the captured programs' own metadata; the step arrays that parts asked for; the cache report."""
-        staging = sum(e[0].numel() * 4 for e in self._staging if e is not None)
+        staging = self._staging.bytes() + self._moves.bytes()
         return {
             **self.counters,
             "execution": self.execution,

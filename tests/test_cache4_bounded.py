@@ -1,0 +1,62 @@
+"""The engine's host side of a bounded number of keys in the cache of 4 bits: what a step leaves for the next while keys are given up, and what
+is refused, without a GPU."""
+import types
+
+import pytest
+import torch
+
+from runtime.config import preset
+from runtime.engine.loading import build_from_config_dict
+
+
+class Event:
+    def record(self):
+        pass
+
+    def synchronize(self):
+        pass
+
+
+@pytest.fixture
+def host_runner(monkeypatch):
+    """Makes ModelRunners whose memory lies on the host and whose kernels do nothing: logits are zeros, evictions are listed."""
+    from runtime.engine import runner as module
+    moved = []
+    for name in ("empty", "zeros"):
+        make = getattr(torch, name)
+        monkeypatch.setattr(torch, name, lambda *a, make=make, pin_memory=False, **kw: make(*a, **kw))
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: "stream")
+    monkeypatch.setattr(torch.cuda, "Event", Event)
+    monkeypatch.setattr(module.ops, "prepare", lambda units: None)
+    monkeypatch.setattr(module.ops, "move_states", lambda storages, source, slot: None)
+    monkeypatch.setattr(module.cache4, "evict", lambda *a: moved.append([t.clone() if isinstance(t, torch.Tensor) else t for t in a[2:7]]))
+
+    def make(pages, page_size=16, max_requests=8, **hold):
+        model = build_from_config_dict(preset("tiny-a"))[2]
+        model.hold_cache(4, **hold)
+        model._max_positions = 8192
+        runner = module.ModelRunner(model, n_pages=pages, page_size=page_size, max_requests=max_requests, device="cpu")
+        runner._forward = lambda ctx, take: torch.zeros(ctx.logit_rows.shape[0], model.vocab_size)
+        return runner, moved
+    return make
+
+
+@pytest.mark.parametrize("requests", [1, 3, 4, 5, 8])
+def test_a_steps_logit_slots_outlive_the_evictions_behind_it(host_runner, requests):
+    """Requests that decode side by side pass their bound in one step.  Tokens are picked afterwards, at the slots that the step's metadata names."""
+    from runtime.engine.runner import StepEntry
+    runner, moved = host_runner(pages=4096, keep=2048, recent=64, slack=64, portion=2112)
+    for r in range(requests):
+        runner.create(r)
+    runner.step([StepEntry(r, [1] * 2112, []) for r in range(requests)])
+    assert not moved
+    runner.step([StepEntry(r, [1], [0]) for r in range(requests)])
+    assert len(moved) == requests and all(runner.cache.cached(r) == 2048 for r in range(requests))
+    wanted, slots, where = runner._last_wanted
+    assert wanted == list(range(requests)) and where.tolist() == slots == [runner.cache.slots.slot_of(r) for r in range(requests)]
+    # and each eviction was told of its own request: keys held, slots, pages
+    for r, (tables, new_tables, lengths, slots, new_slots) in enumerate(moved):
+        assert lengths.tolist() == [2113] and slots.tolist() == new_slots.tolist() == [runner.cache.slots.slot_of(r)]
+        assert new_tables[0].tolist() == runner.cache.table(0, r) and tables.shape == (1, 133)
+    runner.cache.check()
