@@ -247,6 +247,7 @@ class ModelRunner:
                         self._give_up(d.request)
             except BaseException:
                 self._failed.update(e.request for e in entries)      # (pages that hold nothing yet, and logits that nobody got)
+                self._last_wanted = None
                 raise
         self.steps += 1
         self.counters["steps"] += 1

@@ -60,3 +60,24 @@ def test_a_steps_logit_slots_outlive_the_evictions_behind_it(host_runner, reques
         assert lengths.tolist() == [2113] and slots.tolist() == new_slots.tolist() == [runner.cache.slots.slot_of(r)]
         assert new_tables[0].tolist() == runner.cache.table(0, r) and tables.shape == (1, 133)
     runner.cache.check()
+
+
+def test_nothing_is_picked_from_a_step_whose_kept_keys_could_not_be_moved(host_runner, monkeypatch):
+    """The step raises, nobody has its logits: those of an earlier step must not be taken for them."""
+    from runtime.engine import runner as module
+    from runtime.engine.runner import StepEntry
+    runner, _ = host_runner(pages=64, keep=32, recent=8, slack=16, portion=64)
+    runner.create("x")
+    logits = runner.step([StepEntry("x", [1] * 40, [39])])
+
+    def fails(*args):
+        raise module.ops.KernelError("no")
+    monkeypatch.setattr(module.cache4, "evict", fails)
+    with pytest.raises(module.ops.KernelError):
+        runner.step([StepEntry("x", [1] * 20, [19])])
+
+    class Sampler:
+        def pick(self, logits, params, out, index):
+            raise AssertionError("picked")
+    with pytest.raises(ValueError, match="not those of the last step"):
+        runner.pick(Sampler(), logits, [(0.0, 0, 0)])
