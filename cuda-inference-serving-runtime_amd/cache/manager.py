@@ -312,15 +312,25 @@ class CacheManager:
         return out
 
 
-def pages_that_fit(site_needs, page_size, itemsize, free_bytes, fraction=0.8, most=None):
-    """How many pages a pool may have so that the caches of all sites take `fraction` of `free_bytes`:
+def pages_addressable(site_needs, page_size, requests, positions, portion):
+    """How many pages a pool can make use of: those of `requests` requests of `positions` tokens, or, where they keep a bounded number of keys,
+    of the bound with its slack and a step's `portion`, and those that the kept keys of one request move to (CacheManager.give_up)."""
+    keep, slack = max(((getattr(need, "keep", 0), getattr(need, "slack", 0)) for need in site_needs.values()), default=(0, 0))
+    each = -(-positions // page_size)
+    if not keep:
+        return requests * each
+    return requests * min(each, -(-(keep + slack + max(1, portion)) // page_size)) + -(-keep // page_size)
+
+
+def pages_that_fit(site_needs, page_size, itemsize, free_bytes, fraction=0.8, most=None, beside=0):
+    """How many pages a pool may have so that the caches of all sites take `fraction` of `free_bytes`, less `beside` bytes:
     a page index costs, in every site that keeps pages, page_size times the elements its need takes a token.
     `most` caps the answer (more pages than the requests can ever address are of no use)."""
     per_page = sum((need.bytes_per_token(itemsize) if hasattr(need, "bytes_per_token") else need.elements_per_token() * itemsize) * page_size
                    for need in site_needs.values() if need is not None)
     if per_page == 0:
         return 1
-    pages = int(free_bytes * fraction) // per_page
+    pages = int(free_bytes * fraction - beside) // per_page
     if most is not None:
         pages = min(pages, most)
     if pages < 1:

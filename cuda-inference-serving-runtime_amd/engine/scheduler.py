@@ -22,6 +22,7 @@ are the same; a request that ends on an end-of-sequence token is found out one
 step late, and the token it decoded meanwhile is dropped.
 """
 import enum
+import math
 import time
 from collections import deque
 from dataclasses import dataclass, field
@@ -330,27 +331,30 @@ class Engine:
                     keep_keys=0, keep_recent=None, **limits):
         """An engine for the model in `folder` (config.json + safetensors).  Steps run as captured programs unless
         execution="eager" (kernels launched one by one).  pages None (or 0): as many as fit
-        into four fifths of the GPU memory that is free once the weights are loaded, at most what the
-        requests can address.  `cache_bits` 4: the cache holds keys and values in 4 bits; `keep_keys`: and about that many keys a request, those
+        into four fifths of the GPU memory that is free once the weights are loaded (beside the sums that a bounded number of keys is kept by), at
+        most what the requests can address.  `cache_bits` 4: the cache holds keys and values in 4 bits; `keep_keys`: and about that many keys a request, those
         with the most attention weight and the last `keep_recent` (a quarter of them unless given)."""
         import torch
-        from ..cache import pages_that_fit
+        from ..cache import pages_addressable, pages_that_fit
         from .loading import load_model
         from .runner import ModelRunner
         model = load_model(folder, dtype=dtype, device=device)
+        # (what a step brings a request at most: Engine's own limits, see __init__)
+        portion = max(1, min(limits.get("prefill_chunk", 8), limits.get("token_budget", 32)))
         if cache_bits is not None:
-            # (what a step brings a request at most: Engine's own limits, see __init__)
-            portion = max(1, min(limits.get("prefill_chunk", 8), limits.get("token_budget", 32)))
             model.hold_cache(cache_bits, keep_keys, keep_recent, portion=portion)
         elif keep_keys:
             raise ValueError("a bounded number of keys is kept by the cache of 4 bits (cache_bits=4)")
         max_requests = max(8, limits.get("max_active", 8))
         if not pages:
             free, _ = torch.cuda.mem_get_info(torch.device(device))
-            addressable = max_requests * -(-model.max_positions // page_size)
+            needs = model.cache_needs()
+            addressable = pages_addressable(needs, page_size, max_requests, model.max_positions, portion)
+            # (sums of attention weights, a state of every request, beside the pages)
+            sums = sum(4 * max_requests * math.prod(need.shape) for need in model.state_needs().values()) if getattr(model, "kept_keys", None) else 0
             # (the attention kernels address a site's keys with 32-bit byte offsets: fewer than 2^31 elements;
             # a model whose mixers keep no keys has nothing to size)
-            widths = [need.kv_heads * need.head_dim for need in model.cache_needs().values() if need is not None and not hasattr(need, "storage_dtype")]
+            widths = [need.kv_heads * need.head_dim for need in needs.values() if need is not None and not hasattr(need, "storage_dtype")]
             if widths:
                 by_offsets = (2 ** 31 - 1) // (max(widths) * page_size)
                 if by_offsets < addressable:
@@ -358,7 +362,7 @@ class Engine:
                     print(f"[runtime] the pool is limited to {by_offsets} pages a layer by the kernels' 32-bit offsets "
                           f"(the requests could address {addressable})", file=sys.stderr)
                     addressable = by_offsets
-            pages = pages_that_fit(model.cache_needs(), page_size, 2 if dtype == "bfloat16" else 4, free, most=addressable)
+            pages = pages_that_fit(needs, page_size, 2 if dtype == "bfloat16" else 4, free, most=addressable, beside=sums)
         runner = ModelRunner(model, n_pages=pages, page_size=page_size, max_requests=max_requests, device=device,
                              execution=execution)
         return cls(runner, **limits)

@@ -81,3 +81,47 @@ def test_nothing_is_picked_from_a_step_whose_kept_keys_could_not_be_moved(host_r
             raise AssertionError("picked")
     with pytest.raises(ValueError, match="not those of the last step"):
         runner.pick(Sampler(), logits, [(0.0, 0, 0)])
+
+
+@pytest.fixture
+def sized(monkeypatch):
+    """Engine.from_folder on the host: the number of pages that its runner is made with, the memory free for them being `free` bytes."""
+    from runtime.engine import loading, runner as module
+    from runtime.engine.scheduler import Engine
+
+    class Asked(Exception):
+        pass
+
+    def asked(model, n_pages, **kw):
+        raise Asked(n_pages)
+
+    def make(free, positions=8192, name="tiny-a", **kw):
+        model = build_from_config_dict(preset(name))[2]
+        model._max_positions = positions
+        monkeypatch.setattr(loading, "load_model", lambda folder, dtype, device: model)
+        monkeypatch.setattr(torch.cuda, "mem_get_info", lambda device: (free, free))
+        monkeypatch.setattr(module, "ModelRunner", asked)
+        with pytest.raises(Asked) as got:
+            Engine.from_folder("", pages=0, **kw)
+        return got.value.args[0], model
+    return make
+
+
+def test_a_pool_as_large_as_fits_is_no_larger_than_bounded_requests_can_use(sized):
+    """Eight requests of 512 + 64 + 32 keys, and the pages that the kept keys of one move to; all their tokens where nothing bounds them."""
+    most, bounded = 1 << 40, dict(cache_bits=4, keep_keys=512, prefill_chunk=32)
+    assert sized(most, **bounded)[0] == 8 * 38 + 32
+    assert sized(most, page_size=8, max_active=20, **bounded)[0] == 20 * 76 + 64
+    assert sized(most, positions=300, **bounded)[0] == 8 * 19 + 32         # (requests that never reach the bound)
+    assert sized(most, cache_bits=4, prefill_chunk=32)[0] == 8 * 512
+    assert sized(most, prefill_chunk=32)[0] == 8 * 512
+    assert sized(1 << 20, cache_bits=4, prefill_chunk=32)[0] < 8 * 512
+
+
+def test_a_pool_as_large_as_fits_leaves_room_for_the_sums(sized):
+    """The sums of attention weights take memory beside the pages: both together are four fifths of what is free."""
+    free = 1 << 20
+    pages, model = sized(free, cache_bits=4, keep_keys=512, prefill_chunk=32, max_active=32)
+    sums = 32 * sum(4 * need.shape[0] * need.shape[1] for need in model.state_needs().values())
+    page = sum(need.bytes_per_token(2) * 16 for need in model.cache_needs().values())
+    assert sums > free // 4 and pages == int(0.8 * free - sums) // page > 100
