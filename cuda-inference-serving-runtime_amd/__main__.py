@@ -34,7 +34,7 @@ def main(argv=None):
     parser.add_argument("--pages", type=int, default=128, help="cache pages; 0: as many as fit into the free GPU memory")
     parser.add_argument("--page-size", type=int, default=16)
     parser.add_argument("--cache-bits", type=int, choices=[4], help="hold cached keys and values in 4 bits (else in the activations' type)")
-    parser.add_argument("--keep-keys", type=int, default=0, help="with --cache-bits 4: keys a request keeps, those with the most attention weight; 0: all")
+    parser.add_argument("--keep-keys", type=int, default=0, help="with --cache-bits 4: keys a request keeps, those with the most attention weight; 0: all (the move of as many takes spare pages: see --pages)")
     parser.add_argument("--keep-recent", type=int, help="of --keep-keys, the last ones, which stay whatever their weight (a quarter unless given)")
     parser.add_argument("--token-budget", type=int, default=32)
     parser.add_argument("--prefill-chunk", type=int, default=8)

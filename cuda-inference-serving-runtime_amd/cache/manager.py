@@ -118,6 +118,11 @@ class CacheManager:
         """Keys that the request holds (its length, less what it has given up)."""
         return self.lengths[request] - self.dropped.get(request, 0)
 
+    @property
+    def spare(self):
+        """Pages of a group that the kept keys of one request move to (give_up)."""
+        return -(-self.keep // self.page_size)
+
     def overfull(self, request):
         """Whether the request holds more keys than its bound and the slack together."""
         return self.keep > 0 and self.cached(request) > self.keep + self.slack
@@ -126,8 +131,7 @@ class CacheManager:
         """All but `keep` of the request's keys go: per group (old block table, new block table), the pages of the old ones back in the pool.
         The caller moves the kept keys, on the stream that every later user of those pages is ordered behind.  OutOfPages, with nothing
         changed, where the kept keys find no pages."""
-        need = -(-self.keep // self.page_size)
-        if any(len(group.pool.free) < need for group in self.groups):
+        if any(len(group.pool.free) < self.spare for group in self.groups):
             raise OutOfPages("no free KV pages for the keys that stay")
         self.dropped[request] = self.lengths[request] - self.keep
         return [group.exchange(request, self.keep) for group in self.groups]
@@ -282,7 +286,7 @@ class CacheManager:
 
     def capacity(self):
         """Pages of each group's pool that requests can be promised: all but what the kept keys of one request move to (give_up)."""
-        return [g.pool.n_pages - -(-self.keep // self.page_size) for g in self.groups]
+        return [g.pool.n_pages - self.spare for g in self.groups]
 
     def most_pages_held(self, tokens, portion):
         """Per group, the most pages one request holds at any time while it grows to `tokens` cached tokens in

@@ -128,6 +128,9 @@ class Engine:
         kept = getattr(runner.model, "kept_keys", None)
         if kept and min(prefill_chunk, token_budget) > kept[2]:
             raise ValueError(f"prompts in portions of {min(prefill_chunk, token_budget)}: the model's cache was made for at most {kept[2]} (hold_cache)")
+        if kept and min(runner.cache.capacity()) < 1:
+            raise ValueError(f"a pool of {min(g.pool.n_pages for g in runner.cache.groups)} pages of {runner.page_size} holds no request: the move of the {kept[0]} keys that a "
+                             f"request keeps sets {runner.cache.spare} aside (more pages, or 0: as many as fit)")
         self.runner = runner
         self.max_active = 1 if policy == "serial" else min(max_active, runner.max_requests)
         self.token_budget, self.prefill_chunk, self.policy = token_budget, prefill_chunk, policy
@@ -164,7 +167,9 @@ class Engine:
             return f"request {r.key!r} would cache {r.cached_tokens} tokens, the context limit is {self.runner.max_context}"
         need = self.ledger.need(r.cached_tokens)
         if not self.ledger.ever_fits(need):
-            return f"request {r.key!r} needs {need} pages, the pools hold {self.runner.cache.capacity()}: it can never run"
+            spare = self.runner.cache.spare
+            aside = f" ({spare} more are set aside for the move of kept keys)" if spare else ""
+            return f"request {r.key!r} needs {need} pages, the pools hold {self.runner.cache.capacity()}{aside}: it can never run"
         return None
 
     def submit(self, request):

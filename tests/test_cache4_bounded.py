@@ -125,3 +125,32 @@ def test_a_pool_as_large_as_fits_leaves_room_for_the_sums(sized):
     sums = 32 * sum(4 * need.shape[0] * need.shape[1] for need in model.state_needs().values())
     page = sum(need.bytes_per_token(2) * 16 for need in model.cache_needs().values())
     assert sums > free // 4 and pages == int(0.8 * free - sums) // page > 100
+
+
+def test_a_pool_that_the_kept_keys_fill_is_refused_by_name(host_runner):
+    """The pages that one request's kept keys move to are set aside: where that is the whole pool, no request could ever run."""
+    from runtime.engine.scheduler import Engine, Request
+    for pages in (100, 128):
+        with pytest.raises(ValueError, match=f"{pages} pages of 16.*2048 keys.*128"):
+            Engine(host_runner(pages=pages, keep=2048, portion=8)[0])
+    engine = Engine(host_runner(pages=129, keep=2048, portion=8)[0])
+    engine.submit(Request("short", [1] * 10, 6))                          # (15 tokens in the one page left)
+    with pytest.raises(ValueError, match="128 more are set aside"):
+        engine.submit(Request("longer", [1] * 10, 8))
+    Engine(host_runner(pages=1)[0]).submit(Request("all keys", [1] * 10, 6))
+
+
+def test_the_documented_command_takes_requests_of_any_length(sized):
+    """The README's command with a bounded number of keys: its pool holds a request at its bound, whatever the requests' lengths."""
+    import shlex
+    from conftest import ROOT
+    from runtime.cache import CacheManager
+    lines = [line for line in (ROOT / "README.md").read_text().splitlines() if line.startswith("python") and "--keep-keys" in line]
+    assert lines
+    for line in lines:
+        words = shlex.split(line)
+        option = lambda name, default: int(words[words.index(name) + 1]) if name in words else default      # noqa: E731
+        pages, size, chunk = option("--pages", 128), option("--page-size", 16), min(option("--prefill-chunk", 8), option("--token-budget", 32))
+        auto, model = sized(200 << 30, positions=131072, page_size=size, prefill_chunk=chunk, cache_bits=option("--cache-bits", None), keep_keys=option("--keep-keys", 0))
+        cache = CacheManager(model.cache_needs(), pages or auto, size, 8)
+        assert all(most <= left for most, left in zip(cache.most_pages_held(131072, chunk), cache.capacity()))

@@ -24,3 +24,18 @@ def test_requests_of_equal_length_pass_their_bound_together(folders, execution, 
         assert len({e.requests[str(i)].launched for i in range(len(prompts))}) == 1
         outputs.append([e.requests[str(i)].generated for i in range(len(prompts))])
     assert outputs[0] == outputs[1] and all(len(o) == 100 for o in outputs[0])
+
+
+def test_the_command_line_names_a_pool_that_the_kept_keys_fill(folders):
+    import json
+    import os
+    import subprocess
+    import sys
+    from conftest import ROOT
+    env = dict(os.environ, PYTHONPATH=str(ROOT))
+    base = [sys.executable, "-m", "runtime", "--checkpoint", str(folders["c"]), "--tokens", "1,2,3", "--max-new-tokens", "8", "--cache-bits", "4", "--keep-keys", "2048"]
+    out = subprocess.run(base, capture_output=True, text=True, env=env, cwd=ROOT, timeout=100)
+    assert out.returncode != 0 and "128 pages of 16 holds no request" in out.stderr
+    out = subprocess.run(base + ["--pages", "0"], capture_output=True, text=True, env=env, cwd=ROOT, timeout=100)
+    assert out.returncode == 0, out.stderr
+    assert len(json.loads(out.stdout)["requests"][0]["generated"]) == 8
