@@ -123,6 +123,8 @@ class ModelRunner:
                                   state_needs=model.state_needs(), allocate_pages=allocate_pages,
                                   allocate_state=allocate_state, copy_pages=self._copy_pages,
                                   move_states=ops.move_states)
+        if hasattr(model, "runners"):
+            model.runners.add(self)       # (it is not told to hold its cache otherwise from here on)
         self.workspace = Workspace(self.device)
         self.scratch = ops.ScratchPool(ring=not getattr(model, "routes", False))   # what products need beyond their operands (never shared with another runner)
         self.max_context = model.max_positions

@@ -8,6 +8,8 @@ case it keeps no cache and attends to what that entry wrote.  Cache *sites* are
 schedule indices.  The reference's model is the fixed loop of
 runtime/model.py:106-120; here the loop is over the schedule.
 """
+import gc
+import weakref
 from dataclasses import dataclass
 from typing import Optional
 
@@ -51,6 +53,7 @@ class Model:
                                          f"entry {entry.reads} keeps the last {kept.window}")
         self.dtype = None
         self.device = None
+        self.runners = weakref.WeakSet()      # that hold a cache as the mixers said when they were made
 
     # -- weights ------------------------------------------------------------
     def parts(self):
@@ -82,6 +85,10 @@ class Model:
         """Before a runner is made: the cache holds keys and values in 4 bits (kernels/cache4.py).  With `keep` a request holds that many
         keys and at most `slack` more between steps: beyond that, every layer and head gives up the keys with the least attention weight so far, but
         none of the last `recent` (a quarter of `keep` unless given); a step brings a request at most `portion` tokens then."""
+        if self.runners:
+            gc.collect()                      # (a runner that nobody uses may stand in a cycle with its engine)
+            if self.runners:
+                raise ValueError("how the cache is held is said before a runner is made")
         if bits != 4:
             raise ValueError(f"a cache of {bits} bits: 4, or the activations' type")
         recent = keep // 4 if recent is None else recent

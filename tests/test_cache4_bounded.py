@@ -154,3 +154,23 @@ def test_the_documented_command_takes_requests_of_any_length(sized):
         auto, model = sized(200 << 30, positions=131072, page_size=size, prefill_chunk=chunk, cache_bits=option("--cache-bits", None), keep_keys=option("--keep-keys", 0))
         cache = CacheManager(model.cache_needs(), pages or auto, size, 8)
         assert all(most <= left for most, left in zip(cache.most_pages_held(131072, chunk), cache.capacity()))
+
+
+def test_a_cache_is_held_otherwise_only_before_a_runner_has_it(host_runner):
+    """A runner's pages are laid out when it is made; a model whose runners are gone may be told anew."""
+    from runtime.engine import runner as module
+    runner, _ = host_runner(pages=8)
+    model = runner.model
+    for again in (dict(), dict(keep=8)):
+        with pytest.raises(ValueError, match="before a runner"):
+            model.hold_cache(4, **again)
+    assert model.kept_keys is None and all(layer.mixer.four_bits == (0, 64, 2048) for layer in model.layers)
+    del runner
+    model.hold_cache(4, keep=8)
+    assert module.ModelRunner(model, n_pages=8, device="cpu").cache.keep == 8
+    plain = build_from_config_dict(preset("tiny-a"))[2]
+    plain.dtype = torch.float32
+    one = module.ModelRunner(plain, n_pages=8, device="cpu")
+    with pytest.raises(ValueError, match="before a runner"):
+        plain.hold_cache(4)
+    assert one.cache.pages_of_site(0)[1].dtype == torch.float32 and not plain.layers[0].mixer.four_bits
