@@ -97,14 +97,13 @@ class Model:
         mixers = [getattr(layer, "mixer", None) for layer in self.layers]
         if any(not hasattr(mixer, "hold_in_4_bits") for mixer in mixers):
             raise ValueError("a layer whose keys and values cannot be held in 4 bits")
-        done = []
+        held = [getattr(mixer, "four_bits", None) for mixer in mixers]
         try:
             for mixer in mixers:
                 mixer.hold_in_4_bits(keep, slack, portion)
-                done.append(mixer)
         except ValueError:
-            for mixer in done:
-                mixer.four_bits = None
+            for mixer, before in zip(mixers, held):
+                mixer.four_bits = before
             raise
         self.kept_keys = (keep, recent, portion) if keep else None
 

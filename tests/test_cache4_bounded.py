@@ -174,3 +174,15 @@ def test_a_cache_is_held_otherwise_only_before_a_runner_has_it(host_runner):
     with pytest.raises(ValueError, match="before a runner"):
         plain.hold_cache(4)
     assert one.cache.pages_of_site(0)[1].dtype == torch.float32 and not plain.layers[0].mixer.four_bits
+
+
+def test_a_refused_bound_leaves_the_cache_held_as_it_was():
+    model = build_from_config_dict(preset("tiny-a"))[2]
+    model.layers[-1].mixer.window = 8                                     # (holds its keys in 4 bits, but no bounded number of them)
+    with pytest.raises(ValueError, match="without a window"):
+        model.hold_cache(4, keep=8)
+    assert all(layer.mixer.four_bits is None for layer in model.layers) and model.kept_keys is None
+    model.hold_cache(4)
+    with pytest.raises(ValueError, match="without a window"):
+        model.hold_cache(4, keep=8)
+    assert all(layer.mixer.four_bits == (0, 64, 2048) for layer in model.layers) and model.kept_keys is None
