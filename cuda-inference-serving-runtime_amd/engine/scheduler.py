@@ -348,8 +348,8 @@ class Engine:
         portion = max(1, min(limits.get("prefill_chunk", 8), limits.get("token_budget", 32)))
         if cache_bits is not None:
             model.hold_cache(cache_bits, keep_keys, keep_recent, portion=portion)
-        elif keep_keys:
-            raise ValueError("a bounded number of keys is kept by the cache of 4 bits (cache_bits=4)")
+        elif keep_keys or keep_recent is not None:
+            raise ValueError("a bounded number of keys (keep_keys, and keep_recent of them) is kept by the cache of 4 bits (cache_bits=4)")
         max_requests = max(8, limits.get("max_active", 8))
         if not pages:
             free, _ = torch.cuda.mem_get_info(torch.device(device))

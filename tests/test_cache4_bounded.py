@@ -186,3 +186,14 @@ def test_a_refused_bound_leaves_the_cache_held_as_it_was():
     with pytest.raises(ValueError, match="without a window"):
         model.hold_cache(4, keep=8)
     assert all(layer.mixer.four_bits == (0, 64, 2048) for layer in model.layers) and model.kept_keys is None
+
+
+@pytest.mark.parametrize("wrong", [dict(keep_recent=4), dict(keep_recent=0), dict(keep_keys=8), dict(cache_bits=4, keep_recent=4)])
+def test_options_of_a_bound_that_is_not_there_are_refused(monkeypatch, wrong):
+    """`keep_recent` says which of a bounded number of keys stay: without the bound it says nothing."""
+    from runtime.engine import loading, runner as module
+    from runtime.engine.scheduler import Engine
+    monkeypatch.setattr(loading, "load_model", lambda folder, dtype, device: build_from_config_dict(preset("tiny-a"))[2])
+    monkeypatch.setattr(module, "ModelRunner", lambda *a, **kw: pytest.fail("a runner was made"))
+    with pytest.raises(ValueError, match="keep|kept"):
+        Engine.from_folder("", **wrong)
