@@ -110,7 +110,10 @@ def _record(heads, kv_heads, dim, page_size):
         raise KernelError(f"cache4: heads of {dim} in pages of {page_size}: an even size up to {MAX_HEAD}, a power of two from 8 on")
     if kv_heads <= 0 or heads <= 0 or heads % kv_heads:
         raise KernelError(f"cache4: {heads} query heads are not a multiple of {kv_heads} key/value heads")
-    return record_bytes(dim, page_size)
+    record = record_bytes(dim, page_size)
+    if record >= 1 << 31 or kv_heads * record >= 1 << 32:              # (the kernels' offsets within a page)
+        raise KernelError(f"cache4: pages of {page_size} tokens of {kv_heads} heads of {dim} take {kv_heads * record} bytes: fewer than 32 bits can say, and a head's fewer than 31")
+    return record
 
 
 def _gpu_of(t, name, dims):

@@ -197,3 +197,24 @@ def test_options_of_a_bound_that_is_not_there_are_refused(monkeypatch, wrong):
     monkeypatch.setattr(module, "ModelRunner", lambda *a, **kw: pytest.fail("a runner was made"))
     with pytest.raises(ValueError, match="keep|kept"):
         Engine.from_folder("", **wrong)
+
+
+@pytest.mark.parametrize("kv_heads, dim, page_size, fits", [(8, 128, 1 << 21, True), (8, 128, 1 << 22, False), (1, 256, 1 << 22, True), (1, 256, 1 << 23, False),
+                                                            (1, 2, 1 << 25, True), (1, 2, 1 << 26, False), (2, 32, 1 << 25, True), (4, 32, 1 << 25, False)])
+def test_pages_past_32_bits_are_refused(kv_heads, dim, page_size, fits):
+    """A head's page is reckoned in 31 bits and a page of all heads in 32: larger ones would be read from the wrong place.  (Found before anything
+    else of the call, here that its tensors are not on a GPU.)"""
+    from runtime.kernels import cache4
+    from runtime.kernels.ops import KernelError
+    bytes_of = kv_heads * cache4.record_bytes(dim, page_size)
+    assert fits == (bytes_of < 1 << 32 and bytes_of // kv_heads < 1 << 31)
+    none = torch.zeros(1, 1)
+    plan = cache4.plan([1], [0], 2 * kv_heads, kv_heads, dim, device="cpu", state_slots=[0])
+    calls = [(cache4.rope_write, (none, none, none, none, none, none, none, 2 * kv_heads, kv_heads, dim, page_size)),
+             (cache4.read, (none, none, none, none, kv_heads, dim, page_size)),
+             (cache4.attention, (none, none, none, plan, none, 2 * kv_heads, kv_heads, dim, page_size, 0.1)),
+             (cache4.add_weights, (none, none, none, none, plan, none, 2 * kv_heads, kv_heads, dim, page_size, 0.1)),
+             (cache4.evict, (none, [none], none, none, none, none, none, kv_heads, dim, page_size, 8, 2, none))]
+    for call, args in calls:
+        with pytest.raises(KernelError, match="GPU|plan" if fits else "32 bits"):
+            call(*args)
