@@ -244,7 +244,10 @@ def fill_pieces(tasks, merges, counts, cached, rows_per_task, pieces, window, tu
     unused ones at the end; returns how many tasks and merges there are.  Tiles of `rows_per_task` rows of a segment; the keys of long
     ones are cut so that all pieces are about as long as `pieces` of them would be, the longest first; of the second `turn` tasks, which join the
     first on their compute units, the longest last.  (2,048 rows of 9 heads of 64: 21.8 us without that, 20.5 with it; 4,000 rows of 32 heads of
-    128: 307, 296.  Where there are as many tiles as pieces anyway none is cut: 2,048 rows take 18.5 us whole, and 26 when the longer ones are cut.)"""
+    128: 307, 296.)  Cut is what is half as long again as a piece; where there are as many tiles as pieces anyway, what is two and a half times as long: a prompt's
+    last rows have twice the keys of the average, and are better left whole (2,048 rows take 18.5 us, and 26 when the longer ones are cut), but a row behind many
+    keys beside them would be walked by one block a head (with 2,048 rows of 32 heads of 128 one row of 32k keys 869 us whole, 84 cut, one of 4k 116 and 73, 64
+    rows behind 32k 926 and 117; limits of two and a half to four times do alike, where both cut)."""
     counts, cached = np.asarray(counts, dtype=np.int64), np.asarray(cached, dtype=np.int64)
     tiles = -(-counts // rows_per_task)
     n = int(tiles.sum())
@@ -256,7 +259,7 @@ def fill_pieces(tasks, merges, counts, cached, rows_per_task, pieces, window, tu
     first = np.maximum(0, sees - window) // STEP if window else np.zeros(n, dtype=np.int64)
     steps = -(-(sees + rows - 1) // STEP) - first
     each = max(LEAST_PIECE, -(-int(steps.sum()) // pieces))
-    cuts = np.where((2 * steps >= 3 * each) & (n < pieces), -(-steps // each), 1)
+    cuts = np.where(2 * steps >= (3 if n < pieces else 5) * each, -(-steps // each), 1)
     share = -(-steps // cuts)
     cuts = -(-steps // share)
     of = np.repeat(np.arange(n), cuts)

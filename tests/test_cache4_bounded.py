@@ -218,3 +218,18 @@ def test_pages_past_32_bits_are_refused(kv_heads, dim, page_size, fits):
     for call, args in calls:
         with pytest.raises(KernelError, match="GPU|plan" if fits else "32 bits"):
             call(*args)
+
+
+@pytest.mark.parametrize("counts, cached", [([2048, 1], [0, 32767]), ([1024, 1], [0, 32767]), ([2048, 1], [0, 8191]), ([2048] + [1] * 8, [0] + [4095] * 8),
+                                            ([64, 2048], [32768, 0]), ([512, 1600], [16384, 0]), ([300] * 40 + [1], [0] * 40 + [100000])])
+@pytest.mark.parametrize("heads, kv_heads, dim", [(32, 8, 128), (9, 3, 64)])
+def test_long_rows_beside_a_prompt_are_cut(counts, cached, heads, kv_heads, dim):
+    """However many tiles a prompt makes, no task walks keys that would be many pieces: the step would wait for it."""
+    from runtime.kernels import cache4
+    plan = cache4.plan(counts, cached, heads, kv_heads, dim, device="cpu")
+    steps = (plan.tasks[:, 5] - plan.tasks[:, 4]).tolist()
+    pieces = cache4.pieces_for(kv_heads, heads // kv_heads, plan.rows_per_task, plan.form, False)
+    assert max(steps) <= 2.5 * max(cache4.LEAST_PIECE, -(-sum(steps) // pieces)) < max(cached) / 32
+    # and what a prompt brings by itself is not: its last rows have twice the keys of the average
+    alone = cache4.plan([2048], [0], heads, kv_heads, dim, device="cpu")
+    assert alone.merges is None and max((alone.tasks[:, 5] - alone.tasks[:, 4]).tolist()) == 64

@@ -39,3 +39,16 @@ def test_the_command_line_names_a_pool_that_the_kept_keys_fill(folders):
     out = subprocess.run(base + ["--pages", "0"], capture_output=True, text=True, env=env, cwd=ROOT, timeout=100)
     assert out.returncode == 0, out.stderr
     assert len(json.loads(out.stdout)["requests"][0]["generated"]) == 8
+
+
+@pytest.mark.parametrize("form, heads, kv, dim, kind", [(0, 9, 3, 64, "bf16"), (0, 8, 2, 128, "f32"), (1, 8, 2, 128, "bf16"), (2, 8, 2, 128, "bf16"), (2, 9, 3, 64, "bf16"), (0, 2, 1, 256, "bf16")])
+@pytest.mark.parametrize("window", [0, 400])
+def test_long_rows_are_cut_beside_more_tiles_than_pieces(form, heads, kv, dim, kind, window, monkeypatch):
+    """A row behind many keys, and a portion behind as many, beside a prompt whose tiles alone are as many as the pieces asked for."""
+    import test_cache4_gpu as step
+    monkeypatch.setattr(step.cache4(), "LEAST_PIECE", 2)
+    made, plan = [], step.cache4()._plan
+    monkeypatch.setattr(step.cache4(), "_plan", lambda *a: (made.append(plan(*a)), made[-1])[1])
+    step.check_step([300, 1, 9], [0, 1500, 1400], heads, kv, dim, 16, kind, window=window, force=(form, 8))
+    counts = [(made[-1].tasks[:, 0] == seg).sum().item() for seg in range(3)]
+    assert counts[0] >= (3 if form == 2 else 8) and (window or (counts[1] > 2 and made[-1].merges is not None))
