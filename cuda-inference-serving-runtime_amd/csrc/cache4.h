@@ -38,6 +38,6 @@ struct Attn4Call {
 struct Weights4Call {
     hipStream_t stream; const void* q; const float* stats; const uint8_t* pages; const int* tables; const int* segments; float* weights; float* parts;
     long long n_pages;
-    int n_segments, span, heads, kv_heads, dim, page, width, window, capacity, n_slots, shares, blocks, dtype;
+    int n_segments, many, span, heads, kv_heads, dim, page, width, window, capacity, n_slots, shares, blocks, dtype;
     float scale;
 };

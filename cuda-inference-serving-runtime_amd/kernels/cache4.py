@@ -52,7 +52,7 @@ def supported(dim, page_size):
 
 # What an entry point takes: a block of bytes with the stream first, laid out as csrc/cache4.hip and cache4.h say (`cisr_call4_bytes` knows them by
 # their place here).  ctypes converts 20 arguments in 1.3 us, a pointer to 20 that are packed in 0.4.
-_CALLS = {"cisr_write4": "8P10i", "cisr_read4": "5P6i", "cisr_evict4": "8P12i", "cisr_merge4": "6P6i", "cisr_attn4": "9Pq10if", "cisr_weights4": "8Pq13if"}
+_CALLS = {"cisr_write4": "8P10i", "cisr_read4": "5P6i", "cisr_evict4": "8P12i", "cisr_merge4": "6P6i", "cisr_attn4": "9Pq10if", "cisr_weights4": "8Pq14if"}
 
 
 def _entry(name):
@@ -292,16 +292,22 @@ def most_tasks(rows, segments, rows_per_task, pieces):
     return 2 * tiles + pieces, tiles
 
 
-def shares_of(rows, segments, span, group, kv_heads):
-    """Into how many shares the items (a row and a head of the group) of a segment are cut where the keys' attention weights are summed; 0: few
-    items, a wave has them all and walks the keys.  Blocks (128 keys and a share) for three a compute unit, of which two run at once and those of shares that
-no row of is left for leave at once, 256 items a share at least.  (2,048 rows of 9 heads of 64 over 3: 15.6 us with two, 13.5 with three, 16 with four; behind
-2,048 keys 23.4 with two, 24.9 with three; behind 6,144 48 and 43.)"""
-    items = -(-rows * group // segments)
-    if items <= 64:
+FEW_ITEMS = 64             # of a segment: rows times heads of the group (csrc/cache4_attention.inc has the same number)
+
+
+def shares_of(rows, many, span, group, kv_heads):
+    """Into how many shares the items (a row and a head of the group) of a segment are cut where the keys' attention weights are summed, by the `rows` of
+    the longest; 0: every segment has few items, a wave has them all and walks the keys.  Segments of few items beside `many` longer ones are summed that way
+    all the same, by a launch of their own: 480 rows and 31 single ones behind 2k keys, 32 heads over 8 of 128, take 298 us together in waves that have
+    all items and 38 so, 1,024 rows and 32 single ones behind 8k keys 194 in blocks that share keys and 97, 512 rows and one behind 8k 33 and 38.
+    Blocks (128 keys and a share) for three a compute unit, of which two run at once and those of shares that
+    no row of is left for leave at once, 256 items a share at least.  (2,048 rows of 9 heads of 64 over 3: 15.6 us with two, 13.5 with three, 16 with four; behind
+    2,048 keys 23.4 with two, 24.9 with three; behind 6,144 48 and 43.)"""
+    items = rows * group
+    if items <= FEW_ITEMS:
         return 0
-    blocks = -(-span // 128) * kv_heads * segments
-    return max(1, min(3 * COMPUTE_UNITS // blocks, items // 256, 65535 // segments))
+    blocks = -(-span // 128) * kv_heads * max(1, many)
+    return max(1, min(3 * COMPUTE_UNITS // blocks, items // 256, 65535 // max(1, many)))
 
 
 @dataclass(eq=False)
@@ -319,10 +325,12 @@ class Plan:
     tasks: torch.Tensor                # int32 [n, 8]
     merges: Optional[torch.Tensor]     # int32 [m, 4], where keys are in several pieces
     pieces: int = 0                    # pieces that leave partial results, at most
-    segments: Optional[torch.Tensor] = None      # int32 [S, 4]: first row, rows, keys before the first row, state slot
+    segments: Optional[torch.Tensor] = None      # int32 [S, 5], those of most rows first: first row, rows, keys before the first row, state slot, segment
     slots_below: int = 0               # state slots lie below this number
     shares: int = 0                    # see shares_of
     room: Optional[torch.Tensor] = None          # floats for partial results: of `attention` room_of, of `add_weights` parts_of (one after the other)
+    few: bool = False                  # whether a segment has few items
+    many: int = 0                      # segments that have more
 
     def __post_init__(self):
         self.index = self.tasks.get_device()
@@ -337,7 +345,7 @@ class Plan:
 
     @property
     def parts_of(self):
-        return self.shares * self.n_segments * self.kv_heads * self.span if self.shares > 1 else 0
+        return self.shares * self.many * self.kv_heads * self.span if self.shares > 1 else 0
 
 
 def _whole(numbers, name, least, n=None):
@@ -369,22 +377,28 @@ def plan(counts, cached, heads, kv_heads, dim, window=None, device="cuda:0", sta
                  pieces_for(kv_heads, group, per_task, form, decode_only))
 
 
+def _listed(firsts, counts, cached, slots):
+    """int32 [S, 5] of the segments as `add_weights` takes them, those of most rows first."""
+    made = np.stack([firsts, counts, cached, slots, np.arange(len(counts))], 1).astype(np.int32)
+    return made[np.argsort(-made[:, 1], kind="stable")]
+
+
 def _plan(counts, cached, heads, kv_heads, dim, window, device, state_slots, form, per_task, pieces):
-    rows, segments = sum(counts), len(counts)
-    longest = max(c + n for c, n in zip(cached, counts))
+    rows, segments, group = sum(counts), len(counts), heads // kv_heads
+    longest, many = max(c + n for c, n in zip(cached, counts)), sum(c * group > FEW_ITEMS for c in counts)
     tasks, merges = (np.empty((n, k), dtype=np.int32) for n, k in zip(most_tasks(rows, segments, per_task, pieces), (8, 4)))
-    n, m = fill_pieces(tasks, merges, counts, cached, per_task, pieces, window, turn_of(kv_heads, heads // kv_heads, per_task, form))
+    n, m = fill_pieces(tasks, merges, counts, cached, per_task, pieces, window, turn_of(kv_heads, group, per_task, form))
     listed = None
     if state_slots is not None:
         slots = _whole(state_slots, "state slots", 0, segments)
         if len(set(slots)) != segments:
             raise KernelError("cache4.plan: two segments with one state slot")
         firsts = np.concatenate(([0], np.cumsum(counts)[:-1]))
-        listed = torch.from_numpy(np.stack([firsts, counts, cached, slots], 1).astype(np.int32)).to(device)
+        listed = torch.from_numpy(_listed(firsts, counts, cached, slots)).to(device)
     parts = int(tasks[:n, 6].max()) + 1
     return Plan(rows, segments, longest, heads, kv_heads, dim, window, form, per_task, torch.from_numpy(tasks[:n]).to(device),
                 torch.from_numpy(merges[:m]).to(device) if m else None, parts, listed, 0 if listed is None else 1 + max(slots),
-                0 if listed is None else shares_of(rows, segments, longest, heads // kv_heads, kv_heads))
+                0 if listed is None else shares_of(max(counts), many, longest, group, kv_heads), few=many < segments, many=many)
 
 
 def _planned(plan, q, tables, pages, heads, kv_heads, dim, page_size, window, what):
@@ -440,12 +454,12 @@ def add_weights(q, stats, pages, tables, plan, weights, heads, kv_heads, dim, pa
         raise KernelError(f"weights: shape {tuple(weights.shape)} for {kv_heads} heads of {plan.span} keys in {plan.slots_below} slots")
     # Blocks of four waves a segment and key head: as many as reach each a step of keys, and no more than run at once (three a compute unit).
     # 16 rows of 2k keys, 8 key heads: 4, 6, 8, 12 and 17 blocks each (6 is the rule's) take 10.4, 8.7, 11.3, 10.7 and 10.9 us.
-    blocks = max(1, min(-(-plan.span // (4 * STEP)), -(-3 * COMPUTE_UNITS // (kv_heads * plan.n_segments))))
+    blocks = max(1, min(-(-plan.span // (4 * STEP)), -(-3 * COMPUTE_UNITS // (kv_heads * plan.n_segments)))) if plan.few or not plan.shares else 0
     slots, _, capacity = weights.shape
     _launch(_of_size("cisr_weights4_d", dim), index, _t(q, "q", q.dtype, (plan.rows, heads * dim), index, 16),
             _t(stats, "stats", torch.float32, (plan.rows, heads), index), _t(pages, "pages", torch.uint8, (n, kv_heads, record), index, 16),
             _t(tables, "tables", torch.int32, table, index), plan.segments.data_ptr(), _t(weights, "weights", torch.float32, weights.shape, index),
-            0 if plan.shares < 2 else plan.room.data_ptr(), n, plan.n_segments, plan.span, heads, kv_heads, dim, page_size, table[1], plan.window,
+            plan.room.data_ptr() if plan.parts_of else 0, n, plan.n_segments, plan.many, plan.span, heads, kv_heads, dim, page_size, table[1], plan.window,
             capacity, slots, plan.shares, blocks, _DT[q.dtype], _scale(scale))
     return weights
 
@@ -554,18 +568,35 @@ class StepPieces:
 
 @dataclass(frozen=True)
 class StepSegments:
-    """Step array: int32 [S, 4] of first row, rows, keys before the first row and state slot of every segment; no rows pad it."""
+    """Step array: int32 [S, 5] of first row, rows, keys before the first row, state slot and number of every segment, those of most rows first; no rows pad
+    it.  Its launch value is the rows of the longest."""
 
     def words(self, rows, segments):
-        return 4 * segments
+        return 5 * segments
 
     def launch_value(self, batch):
-        return None
+        return max(batch.counts)
 
     def fill(self, out, batch, value):
         out[:] = 0
-        n = len(batch.counts)
-        out[:4 * n] = np.stack([batch.first_row, batch.counts, batch.cached, batch.slots], 1).reshape(-1)
+        out[:5 * len(batch.counts)] = _listed(batch.first_row, batch.counts, batch.cached, batch.slots).reshape(-1)
+
+
+@dataclass(frozen=True)
+class StepItems:
+    """Step array without words whose launch value says how many segments have many items (see shares_of), or with `few` whether one has few."""
+    group: int
+    few: bool
+
+    def words(self, rows, segments):
+        return 0
+
+    def launch_value(self, batch):
+        many = sum(c * self.group > FEW_ITEMS for c in batch.counts)
+        return int(many < len(batch.counts)) if self.few else many
+
+    def fill(self, out, batch, value):
+        pass
 
 
 def step_arrays(heads, kv_heads, dim, window, operand, sums):
@@ -573,7 +604,7 @@ def step_arrays(heads, kv_heads, dim, window, operand, sums):
     if operand is None:
         return []
     pieces = StepPieces(heads, kv_heads, dim, _window(window), operand.dtype is torch.bfloat16)
-    return [pieces, StepForm(pieces)] + ([StepSegments()] if sums else [])
+    return [pieces, StepForm(pieces)] + ([StepSegments(), StepItems(heads // kv_heads, True), StepItems(heads // kv_heads, False)] if sums else [])
 
 
 def attend(ctx, q, pages, view, out, heads, kv_heads, dim, scale, window=None, sums=None):
@@ -586,15 +617,18 @@ def attend(ctx, q, pages, view, out, heads, kv_heads, dim, scale, window=None, s
     most, merges = array.most(ctx.n_rows, ctx.n_segments)
     per_task = 1 if ctx.decode_only else max(1, tile_of(form) // (heads // kv_heads))
     rows, S = ctx.n_rows, ctx.n_segments
-    shares, span, segments = 0, ctx.span_hint, None
+    shares, few, many, span, segments = 0, False, 0, ctx.span_hint, None
     if sums is not None:
-        segments = ctx.step_array(StepSegments())[0].view(S, 4)
+        segments, longest = ctx.step_array(StepSegments())
+        segments = segments.view(S, 5)
+        few, many = (ctx.step_array(StepItems(heads // kv_heads, few))[1] for few in (True, False))
+        many = min(many, S)                                            # (under a captured program, rounded up)
         span = min(span, sums.shape[2])
-        shares = shares_of(rows, S, span, heads // kv_heads, kv_heads)
+        shares = shares_of(longest, many, span, heads // kv_heads, kv_heads)
     pieces = n_tasks if split else 0
-    floats = max(pieces * per_task * heads * (dim + 2), shares * S * kv_heads * span if shares > 1 else 0)
+    floats = max(pieces * per_task * heads * (dim + 2), shares * many * kv_heads * span if shares > 1 else 0)
     plan = Plan(rows, S, span, heads, kv_heads, dim, _window(window), form, per_task, words[:8 * min(n_tasks, most)].view(-1, 8), words[len(words) - 4 * merges:].view(-1, 4) if split else None,
-                pieces, segments, 0 if sums is None else sums.shape[0], shares, ctx.buffer("cache4.room", (floats,), torch.float32) if floats else None)
+                pieces, segments, 0 if sums is None else sums.shape[0], shares, ctx.buffer("cache4.room", (floats,), torch.float32) if floats else None, few > 0, many)
     stats = None if sums is None else ctx.buffer("cache4.stats", (rows, heads), torch.float32)
     attention(q, pages, view.tables, plan, out, heads, kv_heads, dim, view.page_size, scale, window, stats)
     if sums is not None:

@@ -233,3 +233,27 @@ def test_long_rows_beside_a_prompt_are_cut(counts, cached, heads, kv_heads, dim)
     # and what a prompt brings by itself is not: its last rows have twice the keys of the average
     alone = cache4.plan([2048], [0], heads, kv_heads, dim, device="cpu")
     assert alone.merges is None and max((alone.tasks[:, 5] - alone.tasks[:, 4]).tolist()) == 64
+
+
+@pytest.mark.parametrize("heads, kv_heads, dim, counts, cached", [(32, 8, 128, [480] + [1] * 31, 1920), (32, 32, 64, [2000] + [1] * 63, 2000), (9, 3, 64, [1, 300, 1, 5], 100),
+                                                                  (32, 8, 128, [1024] + [1] * 32, 8191)])
+def test_segments_are_summed_by_their_own_number_of_items(heads, kv_heads, dim, counts, cached):
+    """A portion's items are shared by blocks however many single rows stand beside it, and those keep waves of their own."""
+    from runtime.engine.context import Batch
+    from runtime.kernels import cache4
+    plan = cache4.plan(counts, [cached] * len(counts), heads, kv_heads, dim, device="cpu", state_slots=range(len(counts)))
+    assert plan.shares >= 1 and plan.few and plan.many == 1
+    for few in ([1] * 64, [16, 1, 3]):
+        plan = cache4.plan(few, [cached] * len(few), heads, kv_heads, dim, device="cpu", state_slots=range(len(few)))
+        assert plan.shares == 0 and plan.few and plan.many == 0
+    plan = cache4.plan([300, 200], [0, 0], heads, kv_heads, dim, device="cpu", state_slots=[0, 1])
+    assert plan.shares >= 1 and not plan.few and plan.many == 2
+    plan = cache4.plan([3, 70, 1, 100], [5, 6, 7, 8], heads, kv_heads, dim, device="cpu", state_slots=[9, 4, 0, 2])
+    assert plan.segments.tolist() == [[74, 100, 8, 2, 3], [3, 70, 6, 4, 1], [0, 3, 5, 9, 0], [73, 1, 7, 0, 2]]
+    # what an engine's step says of it
+    step = lambda counts: Batch(counts, [0] * len(counts), None, False, {})                        # noqa: E731
+    group = heads // kv_heads
+    _, _, rows, few, many = cache4.step_arrays(heads, kv_heads, dim, None, torch.zeros(1, dtype=torch.bfloat16), True)
+    assert [rows.launch_value(step(c)) for c in (counts, [1, 1], [7])] == [max(counts), 1, 7]
+    batches = [step(c) for c in (counts, [300, 200], [64 // group, 300], [64 // group + 1, 300], [1])]
+    assert [few.launch_value(b) for b in batches] == [1, 0, 1, 0, 1] and [many.launch_value(b) for b in batches] == [1, 2, 1, 2, 0]

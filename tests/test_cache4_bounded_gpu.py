@@ -54,3 +54,32 @@ def test_long_rows_are_cut_beside_more_tiles_than_pieces(form, heads, kv, dim, k
     counts = [(made[-1].tasks[:, 0] == seg).sum().item() for seg in range(3)]
     # (the prompt's tiles walk 5 steps on average, the row 47: over 8 to 75 pieces 17 steps at most a piece, so that the row makes three)
     assert counts[0] >= pieces and (window or (counts[1] > 2 and made[-1].merges is not None))
+
+
+@pytest.mark.parametrize("counts, cached", [([150, 1, 40, 3, 1], [10, 70, 200, 0, 333]), ([1, 16, 17, 64, 65, 1], [5, 0, 90, 130, 31, 2]), ([100, 90], [0, 300])])
+@pytest.mark.parametrize("heads, kv, dim, kind", [(8, 2, 128, "bf16"), (9, 3, 64, "f32"), (4, 4, 64, "bf16"), (3, 1, 20, "bf16"), (40, 1, 32, "bf16"), (2, 1, 256, "bf16")])
+@pytest.mark.parametrize("window", [0, 60])
+def test_sums_of_segments_of_few_and_of_many_items(counts, cached, heads, kv, dim, kind, window):
+    """Either kernel takes its own segments, and together every one once."""
+    from test_cache4_gpu import check_step
+    check_step(counts, cached, heads, kv, dim, 16, kind, window=window, weights=True)
+
+
+@pytest.mark.parametrize("chunk", [16, 20, 40])
+def test_sums_of_mixed_steps_are_alike_however_they_run(folders, chunk):
+    """Portions of 20 rows (60 items) are few, but their captured programs' 32 would be many; those of 40 are many beside decoding rows."""
+    from runtime.engine.scheduler import Engine, Request
+    prompts = [random_tokens(300 + i, n, TINY["c"]["vocab_size"]) for i, n in enumerate([1, 130, 60, 200, 40])]
+    tokens, sums = [], []
+    for execution in ("eager", "graph"):
+        e = Engine.from_folder(folders["c"], dtype="float32", pages=400, page_size=8, execution=execution, policy="decode_first", token_budget=4000, prefill_chunk=chunk,
+                               cache_bits=4, keep_keys=100)
+        for i, p in enumerate(prompts):
+            e.submit(Request(str(i), p, 60))
+        seen = []
+        while e.tick():
+            seen.append({key: sum(e.runner.cache.state_storage[site][e.runner.cache.slots.slot_of(key)].double().sum() for site in (0, 1)).item() for key in e.runner.cache.lengths})
+        tokens.append([e.requests[str(i)].generated for i in range(len(prompts))])
+        sums.append(seen)
+        assert e.runner.counters["evictions_of_keys"] > 0 and (execution == "eager" or e.runner.counters["replays"] > 0)
+    assert tokens[0] == tokens[1] and sums[0] == sums[1]
