@@ -67,7 +67,7 @@ class StepContext:
         self.segments = []        # host: [(request, start, count)]
         self.max_context = 0      # host: largest position + 1 among the rows
         self.decode_only = False  # host: every segment brings exactly one token
-        self.span_hint = 0        # host: context length that sizes attention launches (a bucket under capture)
+        self.span_hint = 0        # host: most keys that a row sees, which size attention launches (a bucket under capture)
         self.arrays = {}          # StepArray -> (int32 device view, launch value): what parts asked the metadata to carry
         self.batch = None         # host: the Batch that the step arrays were filled from
         # A product whose partial sums are still to be added to the residual stream: (rows tensor, partials), set by a

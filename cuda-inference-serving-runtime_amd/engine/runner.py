@@ -353,7 +353,9 @@ class ModelRunner:
         n_want = sum(len(e.want) for e in entries)
         T, S, R = pad if pad is not None else (n_rows, n_seg, n_want)
         # the longest context of the step (a captured program brings the bound of its bucket) sizes the block tables
-        longest = max(s + c for s, c in zip(starts, counts)) if not self.cache.dropped else max(d.start - d.dropped + d.count for d in done)
+        reach = longest = max(s + c for s, c in zip(starts, counts))
+        if self.cache.dropped:
+            longest = max(d.start - d.dropped + d.count for d in done)
         W, G, F = self._width(longest if context is None else context), len(self.cache.groups), self._FIXED
         carried = tuple(self.carried)
         layout = (T, S, R, W, carried)
@@ -437,7 +439,7 @@ class ModelRunner:
         ctx.arrays = {array: (view(F + 2 * G + i), batch.launch_values[array]) for i, array in enumerate(carried)}
         self._last_wanted = ([entries[s].request for s in wanted_seg], wanted_slots, view(8)[:n_want])
         ctx.segments = [(d.request, d.start, d.count) for d in done]
-        ctx.max_context = ctx.span_hint = longest
+        ctx.max_context, ctx.span_hint = reach, longest
         ctx.decode_only = decode_only
         return ctx
 

@@ -257,3 +257,16 @@ def test_segments_are_summed_by_their_own_number_of_items(heads, kv_heads, dim, 
     assert [rows.launch_value(step(c)) for c in (counts, [1, 1], [7])] == [max(counts), 1, 7]
     batches = [step(c) for c in (counts, [300, 200], [64 // group, 300], [64 // group + 1, 300], [1])]
     assert [few.launch_value(b) for b in batches] == [1, 0, 1, 0, 1] and [many.launch_value(b) for b in batches] == [1, 2, 1, 2, 0]
+
+
+def test_a_step_tells_its_largest_position_apart_from_its_most_keys(host_runner):
+    """Positions go on counting where keys are given up: what sizes launches over keys is not what positions reach."""
+    from runtime.engine.runner import StepEntry
+    runner, _ = host_runner(pages=64, keep=32, recent=8, slack=16, portion=64)
+    seen = []
+    runner._forward = lambda ctx, take: seen.append((ctx.max_context, ctx.span_hint, int(ctx.positions.max()) + 1))
+    runner.create("x"), runner.create("y")
+    runner.step([StepEntry("x", [1] * 60, []), StepEntry("y", [1] * 9, [])])
+    runner.step([StepEntry("x", [1], []), StepEntry("y", [1], [])])
+    runner.step([StepEntry("y", [1], [])])
+    assert seen == [(60, 60, 60), (61, 33, 61), (11, 11, 11)]
