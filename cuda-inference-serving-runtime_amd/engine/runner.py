@@ -112,6 +112,9 @@ class ModelRunner:
         if len(held) > 1:
             raise ValueError("layers that hold their caches in different types")
         stored = torch.uint8 if held == {"uint8"} else dtype
+        if stored is torch.uint8:
+            for need in needs.values():
+                cache4.check_pages(need.kv_heads, need.head_dim, page_size)
 
         def allocate_pages(shape):
             return torch.zeros(shape, dtype=stored, device=self.device)

@@ -116,6 +116,11 @@ def _record(heads, kv_heads, dim, page_size):
     return record
 
 
+def check_pages(kv_heads, dim, page_size):
+    """Refuses pages that the kernels do not take."""
+    _record(kv_heads, kv_heads, dim, page_size)
+
+
 def _gpu_of(t, name, dims):
     """The index of the GPU that tensor `t`, of so many dimensions, is on."""
     if not isinstance(t, torch.Tensor) or t.dim() != dims or not t.is_cuda:

@@ -270,3 +270,11 @@ def test_a_step_tells_its_largest_position_apart_from_its_most_keys(host_runner)
     runner.step([StepEntry("x", [1], []), StepEntry("y", [1], [])])
     runner.step([StepEntry("y", [1], [])])
     assert seen == [(60, 60, 60), (61, 33, 61), (11, 11, 11)]
+
+
+@pytest.mark.parametrize("page_size", [4, 24, 1 << 26])
+def test_pages_that_the_kernels_do_not_take_are_refused_with_the_runner(host_runner, page_size):
+    """Not by every request's first step."""
+    from runtime.kernels.ops import KernelError
+    with pytest.raises(KernelError, match="pages of"):
+        host_runner(pages=1, page_size=page_size)
