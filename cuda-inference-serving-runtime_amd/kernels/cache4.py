@@ -228,7 +228,7 @@ def launch_of(rows, segments, decode_only, heads, kv_heads, dim, dtype):
     waves share the keys; form 2: four waves of 32 items that walk the keys side by side.
     Microseconds by form, 0 / 1 / 2: 1,024 rows of 9 heads of 64 10 / 14 / 27, 2,048 rows 20 / 19 / 32, 8,192 rows 206 / 158 / 182; 512 rows of 32 heads of 128
     17 / 15 / 24, 1,024 rows 33 / 34 / 46, 1,536 rows 58 / 56 / 59, 2,048 rows 92 / 81 / 77, 4,096 rows 290 / 235 / 196; 4,096 rows of 24 heads of 96
-    219 / 184 / 145; 8,192 rows of 16 heads of 64 329 / 250 / 225."""
+    219 / 184 / 145; 8,192 rows of 16 heads of 64 329 / 250 / 225.  (Small heads change over earlier than the rule says: 4,096 rows of 32 heads of 32 123 / 91 / 83.)"""
     group = heads // kv_heads
     form = 0
     if not decode_only and dtype == torch.bfloat16 and padded(dim) <= 128:
@@ -252,7 +252,8 @@ def fill_pieces(tasks, merges, counts, cached, rows_per_task, pieces, window, tu
     128: 307, 296.)  Cut is what is half as long again as a piece; where there are as many tiles as pieces anyway, what is two and a half times as long: a prompt's
     last rows have twice the keys of the average, and are better left whole (2,048 rows take 18.5 us, and 26 when the longer ones are cut), but a row behind many
     keys beside them would be walked by one block a head (with 2,048 rows of 32 heads of 128 one row of 32k keys 869 us whole, 84 cut, one of 4k 116 and 73, 64
-    rows behind 32k 926 and 117; limits of two and a half to four times do alike, where both cut)."""
+    rows behind 32k 926 and 117; limits of two and a half to four times do alike, where both cut).  Where the rest of the step hides the longer rows, the merge is
+    lost: 250 single rows of 500 keys and six of 4k take 36 us whole and 40 cut."""
     counts, cached = np.asarray(counts, dtype=np.int64), np.asarray(cached, dtype=np.int64)
     tiles = -(-counts // rows_per_task)
     n = int(tiles.sum())
